@@ -183,6 +183,23 @@ int ns2_linear_f16w_tiled(const uint16_t* At, const uint16_t* Wt, const float* b
  * ns2_linear_f16w_tiled (round to nearest even; N % 64 == 0, K % 64 == 0). Done once at load. */
 int ns2_tile_bf16_weight(const uint16_t* W, uint16_t* Wt, int N, int K);
 
+/* 4-bit weights with group scales: W[n,k] = scale[n, k / group] * (code[n,k] - 8), codes 0..15 two
+ * to a byte (W uint8 [N, K/2], the even column in the low four bits), scale fp16 [N, K/group],
+ * group 32, 64 or 128, K % group == 0. The same epilogue as above. a_fmt = 0: A is fp32, = 1: fp16
+ * ([M, lda]). The products are exact (an fp32 activation takes part as a sum of fp16 parts that
+ * keeps 22 of its bits) and summed in fp32, so the result is that of an fp32 linear on the weights
+ * that the codes stand for; an fp32 activation beyond fp16's range (65504) is not taken. Made for the
+ * few rows of single tokens and conditioning vectors; any M runs. Rows of A and W 16-byte aligned.
+ * No counterpart in the reference. */
+int ns2_linear_i4(const void* A, int a_fmt, int lda, const uint8_t* W, const uint16_t* scale,
+                  const float* bias, const float* add, float* C, int M, int N, int K, int group,
+                  int ldc, long long cOff, float alpha, int act, int resid, const float* gate,
+                  long long gOff);
+/* A bf16 weight [N, K] as such 4-bit codes and scales: scale = half(max|w| / 7) of the group,
+ * code = 8 + clamp(rint(w / scale), -7, 7), 8 where the scale is 0. A group that holds a NaN or an
+ * infinity gets a NaN scale. Done once when the weight is loaded. */
+int ns2_quantize_i4(const uint16_t* W, uint8_t* codes, uint16_t* scale, int N, int K, int group);
+
 /* ---- LoRA side path (ops.linear with W.lora, app/gpu/ops.js:50-87 loraDelta; app/lora.js) ---
  * The _lora variants compute the same linear plus the low-rank term
  *   r += sum_k t[m,k] lora_b[n,k],  t = x lora_a^T,
@@ -245,6 +262,49 @@ int ns2_attention_rows_f16kv(const float* q, const uint16_t* k, const uint16_t* 
 int ns2_attention_rows_f16kv_oproj(const float* q, const uint16_t* k, const uint16_t* v, const uint16_t* wo_tiled,
                                    float* part, int Lq, int Lk, int H, int D, int ldq, int ldk, int ldv,
                                    long long qOff, long long kOff, long long vOff, int group, int causal, int N);
+
+/* ---- attention over a key/value cache ----------------------------------------------------
+ * The Gemma3 layers as tokens arrive (app/models/gemma3.js:62-73: head norms and RoPE, then causal
+ * attention, which the reference computes for whole prompts only), with the sliding window that
+ * its local layers have in longer sequences. No counterpart in the reference.
+ *
+ * `batch` sequences bring L new tokens each, rows b*L + i. pos[b*L + i] is the row's position in
+ * its sequence, a device array, so that a recorded graph serves every step; a row whose position
+ * is negative or not below cap is padding: it is read nowhere, and its outputs keep what they hold.
+ * Cache row (b, j, g), position j < cap and K/V head g < KH, is the D values from b*kvBatch +
+ * j*ldkv + g*D on (counted in values, in k and v alike). k_groups == v_groups == NULL: k, v are fp16.
+ * Else k, v hold 4-bit codes, two to a byte (value 2i in the low four bits of byte i), and k_groups,
+ * v_groups an fp16 step s and offset o (2 halfs) per 32 values; such a cache stands for the fp16
+ * values half(o + code * s). D is 64, 96, 128 or 256. q_fmt is the type of q (and o): 0 fp32, 1 fp16.
+ * Rows of X, q, o and the cache are 16-byte aligned (ldkv, kvBatch multiples of 8 for fp16, of 32
+ * for 4 bits).
+ *
+ * ns2_head_norm_cache: X fp32 [batch*L, ldx] holds H query heads, KH key heads and KH value heads
+ * (a q|k|v product). Query and key heads are RMS-normed with w_q / w_k [D] (NULL: not normed) and,
+ * for positions below rope_rows, rotated by the table cs at their position (ns2_head_norm's
+ * layout; NULL: not rotated). Queries go to q [batch*L, ldq] (q may be X itself), keys and values
+ * into the cache at their rows' positions, which have to differ within a sequence. A 4-bit group
+ * takes o = half(least value), s = half(range / 15), code = clamp(rint((x - o) / s), 0, 15); a group
+ * that holds a NaN or an infinity reads as NaN. The sequences' caches must not overlap.
+ *
+ * ns2_attention_cache: for each row at position p, head h and g = h / (H / KH),
+ *   o[row*ldo + h*D ..] = sum_j softmax_j(scale * <q_row,h, k_j,g>) v_j,g over the keys j <= p with
+ *   j < sinks or j > p - window (window = 0: all j <= p).
+ * What the cache holds at other positions, infinities and NaN too, does not matter. kvBatch = 0 lets
+ * all sequences read one cache. fp16 q: the softmax weights are rounded to fp16 for the second
+ * product; fp32 q: queries and weights take part as sums of fp16 parts that keep 22 of their bits
+ * (a query times `scale` must lie in fp16's range). Sums and softmax statistics are fp32. work:
+ * ns2_attention_cache_bytes bytes of device memory that the call may write (NULL where that is 0);
+ * calls that may overlap take one each. */
+int ns2_head_norm_cache(const float* X, int ldx, const int* pos, const float* w_q, const float* w_k,
+                        const float* cs, long long sin_off, int rope_rows, float eps, void* q,
+                        int q_fmt, int ldq, void* k, void* v, uint16_t* k_groups, uint16_t* v_groups,
+                        int batch, int L, int H, int KH, int D, int cap, int ldkv, long long kvBatch);
+size_t ns2_attention_cache_bytes(int batch, int L, int H, int KH, int D, int cap, int window, int sinks);
+int ns2_attention_cache(const void* q, int q_fmt, int ldq, const int* pos, const void* k, const void* v,
+                        const uint16_t* k_groups, const uint16_t* v_groups, void* o, int ldo, int batch,
+                        int L, int H, int KH, int D, int cap, int ldkv, long long kvBatch, int window,
+                        int sinks, float scale, void* work, size_t work_bytes);
 
 /* ---- attention (ops.attention, app/gpu/ops.js:199-209; flashAttentionShader,
  *      app/gpu/kernels.js:119-305) ----------------------------------------------------------

@@ -100,6 +100,14 @@ SIGNATURES = {
     "ns2_linear_f16w_tiled_head_norm_f16kv": [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_int, c_vp, c_int,
                                               c_int, c_vp, c_ll, c_int, c_float, c_vp, c_int],
     "ns2_linear_f16w_tiled_glu_down": [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, c_int, c_vp],
+    "ns2_linear_i4": [c_vp, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_ll, c_float,
+                      c_int, c_int, c_vp, c_ll],
+    "ns2_quantize_i4": [c_vp, c_vp, c_vp, c_int, c_int, c_int],
+    "ns2_head_norm_cache": [c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_ll, c_int, c_float, c_vp, c_int, c_int, c_vp, c_vp,
+                            c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_ll],
+    "ns2_attention_cache_bytes": [c_int] * 8,
+    "ns2_attention_cache": [c_vp, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int,
+                            c_int, c_int, c_int, c_ll, c_int, c_int, c_float, c_vp, c_size],
     "ns2_head_norm": [c_vp, c_vp, c_int, c_int, c_int, c_int, c_ll, c_ll, c_vp, c_ll, c_float],
     "ns2_head_norm2": [c_vp, c_vp, c_int, c_vp, c_int, c_int, c_int, c_int, c_ll, c_ll, c_vp, c_ll, c_float],
     "ns2_norm_mod": [c_vp, c_vp, c_ll, c_ll, c_int, c_int, c_vp, c_float, c_vp],
@@ -122,7 +130,7 @@ SIGNATURES = {
     "ns2_linear_bf16_add_rmsnorm": [c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_float],
 }
 _RESTYPES = {"ns2_last_error": ctypes.c_char_p, "ns2_get_stream": c_vp, "ns2_pool_round": c_size,
-             "ns2_attention_vpack_bytes": c_size}
+             "ns2_attention_vpack_bytes": c_size, "ns2_attention_cache_bytes": c_size}
 
 
 class NS2Error(RuntimeError):
@@ -285,6 +293,15 @@ class Lib:
                 N if ldc is None else ldc, cOff, alpha, ACT[act], int(resid), _ptr(gate), gOff]
         self._linear("ns2_linear_bf16", args, lora)
 
+    def quantize_i4(self, W, codes, scale, N, K, group):
+        self.call("ns2_quantize_i4", _ptr(W), _ptr(codes), _ptr(scale), N, K, group)
+
+    def linear_i4(self, A, a_fmt, lda, W, scale, C, M, N, K, group, *, bias=None, add=None, ldc=None, cOff=0,
+                  alpha=1.0, act="none", resid=False, gate=None, gOff=0):
+        """4-bit weights (W codes [N, K/2], fp16 scale [N, K/group]); a_fmt 0: fp32 A, 1: fp16 A."""
+        self.call("ns2_linear_i4", _ptr(A), a_fmt, lda, _ptr(W), _ptr(scale), _ptr(bias), _ptr(add), _ptr(C), M, N, K,
+                  group, N if ldc is None else ldc, cOff, alpha, ACT[act], int(resid), _ptr(gate), gOff)
+
     def _linear(self, name, args, lora):
         if lora is None:
             self.call(name, *args)
@@ -362,6 +379,26 @@ class Lib:
         """attention_rows with fp16 k and v (their strides and offsets in fp16 elements)."""
         self.call("ns2_attention_rows_f16kv", _ptr(q), _ptr(k), _ptr(v), _ptr(o), Lq, Lk, H, D, ldq, ldk, ldv,
                   ldo, qOff, kOff, vOff, group, int(causal))
+
+    def head_norm_cache(self, X, pos, q, k, v, *, batch, L, H, KH, D, ldx, ldq, cap, ldkv, kvBatch, w_q=None, w_k=None,
+                        cs=None, sin_off=0, rope_rows=0, eps=1e-6, q_fmt=0, k_groups=None, v_groups=None):
+        """New tokens into a key/value cache: 4-bit with k_groups and v_groups, else fp16."""
+        self.call("ns2_head_norm_cache", _ptr(X), ldx, _ptr(pos), _ptr(w_q), _ptr(w_k), _ptr(cs), sin_off, rope_rows, eps,
+                  _ptr(q), q_fmt, ldq, _ptr(k), _ptr(v), _ptr(k_groups), _ptr(v_groups), batch, L, H, KH, D, cap, ldkv,
+                  kvBatch)
+
+    def attention_cache_bytes(self, batch, L, H, KH, D, cap, window=0, sinks=0):
+        return int(self.dll.ns2_attention_cache_bytes(batch, L, H, KH, D, cap, window, sinks))
+
+    def attention_cache(self, q, pos, k, v, o, *, batch, L, H, KH, D, ldq, ldo, cap, ldkv, kvBatch, window=0, sinks=0,
+                        scale=None, q_fmt=0, k_groups=None, v_groups=None, work=None):
+        """Attention of the rows at positions pos over a cache; work: a tensor of attention_cache_bytes bytes
+        or more, or None where that is 0."""
+        if scale is None:
+            scale = 1.0 / D ** 0.5
+        self.call("ns2_attention_cache", _ptr(q), q_fmt, ldq, _ptr(pos), _ptr(k), _ptr(v), _ptr(k_groups),
+                  _ptr(v_groups), _ptr(o), ldo, batch, L, H, KH, D, cap, ldkv, kvBatch, window, sinks, scale, _ptr(work),
+                  0 if work is None else work.numel() * work.element_size())
 
     def head_norm(self, X, w, L, H, D, ld, colOff=0, rowOff=0, cs=None, sinOff=0, eps=1e-6):
         self.call("ns2_head_norm", _ptr(X), _ptr(w), L, H, D, ld, colOff, rowOff, _ptr(cs), sinOff, eps)

@@ -1,0 +1,526 @@
+"""Tokens entering a key/value cache and attention over it (ns2_head_norm_cache, ns2_attention_cache) against their
+definitions in 64 bits: head layouts, fp16 and 4-bit caches, fp32 and fp16 queries, windows, sinks, lengths from one
+token on, padding rows, stale cache rows, strides, refusals, graphs and streams."""
+
+import math
+
+import pytest
+import torch
+
+import cache_reference as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+EPS = 1e-6
+
+
+def gen(seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return lambda *shape: torch.randn(*shape, generator=g, device=DEV)
+
+
+def positions(spans, L):
+    pos = torch.full((len(spans), L), -1, dtype=torch.int32)
+    for b, (s, n) in enumerate(spans):
+        pos[b, :n] = torch.arange(s, s + n, dtype=torch.int32)
+    return pos.to(DEV)
+
+
+# ---- attention ----------------------------------------------------------------------------------
+
+class Cache:
+    """A cache of `batch` sequences with its own strides; values as float64, stale rows poisoned."""
+
+    def __init__(self, rnd, batch, cap, KH, D, i4, pad_row=0, pad_seq=0):
+        self.batch, self.cap, self.KH, self.D, self.i4 = batch, cap, KH, D, i4
+        self.ldkv, self.kvBatch = KH * D + pad_row, cap * (KH * D + pad_row) + pad_seq
+        size = batch * self.kvBatch
+        self.raw, self.groups, self.value = {}, {"k": None, "v": None}, {}
+        for name in "kv":
+            x = rnd(batch, cap, KH, D)
+            if i4:
+                self.raw[name] = torch.zeros(size // 2, dtype=torch.uint8, device=DEV)
+                self.groups[name] = torch.zeros(size // 32, 2, dtype=torch.float16, device=DEV)
+                codes, groups = R.cache_codes(x)
+                self.view(self.raw[name], 2).copy_(codes)
+                self.group_view(name).copy_(groups)
+                self.value[name] = R.cache_values(codes, groups)
+            else:
+                self.raw[name] = torch.zeros(size, dtype=torch.float16, device=DEV)
+                self.view(self.raw[name], 1).copy_(x.half())
+                self.value[name] = x.half().double()
+
+    def view(self, t, per):
+        return torch.as_strided(t, (self.batch, self.cap, self.KH, self.D // per),
+                                (self.kvBatch // per, self.ldkv // per, self.D // per, 1))
+
+    def group_view(self, name):
+        return torch.as_strided(self.groups[name], (self.batch, self.cap, self.KH, self.D // 32, 2),
+                                (self.kvBatch // 16, self.ldkv // 16, self.D // 16, 2, 1))
+
+    def poison(self, b, rows):
+        """What an earlier sequence may have left in rows nobody sees."""
+        for name in "kv":
+            t = self.group_view(name)[b, rows] if self.i4 else self.view(self.raw[name], 1)[b, rows]
+            t[0::3], t[1::3], t[2::3] = math.inf, math.nan, -65504.0
+
+    def args(self):
+        return dict(cap=self.cap, ldkv=self.ldkv, kvBatch=self.kvBatch, KH=self.KH, D=self.D, batch=self.batch,
+                    k_groups=self.groups["k"], v_groups=self.groups["v"])
+
+
+def attend(lib, cache, q, pos, window, sinks, fp16, pad=0, scale=None, o=None):
+    """q [B, L, H, D] float; returns o [B, L, H, D] (rows of padding keep 7)."""
+    B, L, H, D = q.shape
+    ld = H * D + pad
+    dt = torch.float16 if fp16 else torch.float32
+    qb = torch.full((B * L, ld), 3.0, dtype=dt, device=DEV)
+    qb[:, : H * D] = q.reshape(B * L, H * D).to(dt)
+    ob = torch.full((B * L + 2, ld), 7.0, dtype=dt, device=DEV)
+    need = lib.attention_cache_bytes(B, L, H, cache.KH, D, cache.cap, window, sinks)
+    work = torch.full((need + 64,), 255, dtype=torch.uint8, device=DEV)
+    a = cache.args()
+    a["batch"] = B
+    lib.attention_cache(qb, pos, cache.raw["k"], cache.raw["v"], ob, L=L, H=H, ldq=ld, ldo=ld, window=window, sinks=sinks,
+                        scale=scale, q_fmt=int(fp16), work=work[:need] if need else None, **a)
+    torch.cuda.synchronize()
+    assert (work[need:] == 255).all(), "bytes behind the work memory were written"
+    assert (ob[:, H * D:] == 7).all() and (ob[B * L:] == 7).all(), "values outside the rows were written"
+    return ob[: B * L, : H * D].reshape(B, L, H, D)
+
+
+def check(got, q, pos, cache, window, sinks, fp16, what, scale=None):
+    D = q.shape[-1]
+    qd = (q.half() if fp16 else q.float()).double()
+    ref, vmax, smax, n = R.attention(qd, pos, cache.value["k"], cache.value["v"], window, sinks, scale or 1 / math.sqrt(D))
+    live = (pos >= 0) & (pos < cache.cap)
+    bound = R.attention_bound(ref, vmax, smax, n, D, fp16)[live]
+    assert (got[~live] == 7).all(), f"{what}: padding rows were written"
+    err = (got[live].double() - ref[live]).abs()
+    print(f"[parity] {what}: largest error / bound {(err / bound).max().item():.3f}", flush=True)
+    assert torch.isfinite(got[live]).all() and (err <= bound).all(), what
+
+
+HEADS = [(4, 1, 256), (16, 16, 96), (8, 2, 128), (6, 2, 64), (5, 1, 64), (3, 1, 128), (20, 1, 96), (1, 1, 256), (40, 2, 64)]
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("H,KH,D", HEADS)
+def test_single_tokens(ns2lib, H, KH, D, i4, fp16):
+    """One token per sequence: the first token of all, ends of tiles, a full cache, a padding row, one past the cache."""
+    pos = torch.tensor([[0], [1], [15], [31], [32], [63], [64], [199], [-1], [200], [130]], dtype=torch.int32, device=DEV)
+    rnd = gen(H * D)
+    for window, sinks in ((0, 0), (1, 0), (1, 2), (33, 4), (64, 0), (150, 70), (500, 500)):
+        cache = Cache(rnd, len(pos), 200, KH, D, i4)
+        for b in range(len(pos)):
+            p = int(pos[b])
+            cache.poison(b, slice(max(0, p + 1), None))
+            if window and p - window + 1 > sinks:
+                cache.poison(b, slice(sinks, p - window + 1))
+        q = rnd(len(pos), 1, H, D)
+        check(attend(ns2lib, cache, q, pos, window, sinks, fp16), q, pos, cache, window, sinks, fp16,
+              f"step {H}/{KH}x{D} i4={i4} fp16={fp16} window {window} sinks {sinks}")
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("H,KH,D", HEADS)
+@pytest.mark.parametrize("L,start", [(2, 0), (17, 3), (70, 0), (129, 61)])
+def test_prompts(ns2lib, H, KH, D, i4, fp16, L, start):
+    """Several tokens at once, unequal lengths with padding rows, keys before them in the cache."""
+    spans = [(start, L), (start // 2, max(1, L // 3)), (start, L - 1)]
+    pos = positions(spans, L)
+    rnd = gen(L + H * D)
+    for window, sinks in ((0, 0), (7, 2), (64, 1), (40, 100)):
+        cache = Cache(rnd, 3, 200, KH, D, i4)
+        for b, (s, n) in enumerate(spans):
+            cache.poison(b, slice(s + n, None))
+            if window and s - window + 1 > sinks:
+                cache.poison(b, slice(sinks, s - window + 1))
+        q = rnd(3, L, H, D)
+        check(attend(ns2lib, cache, q, pos, window, sinks, fp16), q, pos, cache, window, sinks, fp16,
+              f"prompt {L} from {start} {H}/{KH}x{D} i4={i4} fp16={fp16} window {window} sinks {sinks}")
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+def test_later_tokens_do_not_reach_earlier_ones(ns2lib, D, i4, fp16):
+    """Infinities and NaN in one token's key and value: rows before it, and rows whose window has passed it, are
+    those of a cache without them, in the same call."""
+    L, bad, window = 150, 70, 30
+    pos = positions([(0, L)], L)
+    rnd = gen(D)
+    cache = Cache(rnd, 1, 160, 2, D, i4)
+    q = rnd(1, L, 8, D)
+    clean = attend(ns2lib, cache, q, pos, window, 2, fp16)
+    cache.poison(0, slice(bad, bad + 2))
+    got = attend(ns2lib, cache, q, pos, window, 2, fp16)
+    far = torch.ones(L, dtype=torch.bool, device=DEV)
+    far[bad: bad + 1 + window] = False
+    check(torch.where(far[None, :, None, None], got, clean), q, pos, cache, window, 2, fp16, f"D={D} i4={i4} fp16={fp16}")
+    assert not torch.isfinite(got[0, bad: bad + window]).any(-1).any(), "a visible NaN was lost"
+
+
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("L", [1, 40])
+def test_any_positions(ns2lib, L, i4):
+    """Rows in any order, some at the same position, some of them padding."""
+    g = torch.Generator().manual_seed(L)
+    pos = torch.randint(-40, 330, (2, L), generator=g, dtype=torch.int32).to(DEV)
+    rnd = gen(L)
+    cache = Cache(rnd, 2, 300, 2, 64, i4)
+    q = rnd(2, L, 4, 64)
+    for window, sinks in ((0, 0), (50, 3)):
+        check(attend(ns2lib, cache, q, pos, window, sinks, False), q, pos, cache, window, sinks, False, f"any {L} i4={i4}")
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("L", [1, 35])
+def test_strides(ns2lib, L, i4, fp16):
+    """Rows of q and o wider than the heads, gaps between cache rows and between sequences."""
+    pos = positions([(90, L), (3, L)], L)
+    rnd = gen(11)
+    cache = Cache(rnd, 2, 140, 2, 96, i4, pad_row=32, pad_seq=64)
+    q = rnd(2, L, 6, 96)
+    check(attend(ns2lib, cache, q, pos, 60, 4, fp16, pad=8), q, pos, cache, 60, 4, fp16, f"strides {L} i4={i4} fp16={fp16}")
+
+
+@pytest.mark.parametrize("L", [1, 33])
+def test_one_cache_for_all(ns2lib, L):
+    """kvBatch = 0: every sequence reads the same cached rows."""
+    rnd = gen(12)
+    cache = Cache(rnd, 1, 140, 1, 128, False)
+    pos = positions([(100, L), (20, L), (0, L)], L)
+    q = rnd(3, L, 4, 128)
+    cache.kvBatch = 0
+    got = attend(ns2lib, cache, q, pos, 0, 0, False)
+    for name in "kv":
+        cache.value[name] = cache.value[name].expand(3, -1, -1, -1)
+    check(got, q, pos, cache, 0, 0, False, f"shared {L}")
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("i4", [False, True])
+def test_long_caches(ns2lib, i4, fp16):
+    """Thousands of keys for one token and for a few."""
+    for L, B, (H, KH, D) in ((1, 3, (4, 1, 256)), (5, 2, (8, 2, 128)), (1, 1, (16, 16, 96)), (66, 1, (2, 1, 64))):
+        rnd = gen(D)
+        cap = 6000
+        spans = [(cap - L - 211 * b, L) for b in range(B)]
+        pos = positions(spans, L)
+        cache = Cache(rnd, B, cap, KH, D, i4)
+        q = rnd(B, L, H, D)
+        for window, sinks in ((0, 0), (3333, 100)):
+            check(attend(ns2lib, cache, q, pos, window, sinks, fp16), q, pos, cache, window, sinks, fp16,
+                  f"long {L} {H}/{KH}x{D} i4={i4} fp16={fp16} window {window}")
+
+
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("L", [1, 20])
+def test_offsets_past_32_bits(ns2lib, L, i4):
+    """Cache rows more than 2^32 values into the buffer."""
+    rnd = gen(13)
+    ld, cap, D = 1 << 23, 600, 64
+    small = Cache(rnd, 1, cap, 1, D, i4)
+    big = Cache.__new__(Cache)
+    big.__dict__.update(small.__dict__)
+    big.ldkv, big.kvBatch, size = ld, cap * ld, (cap - 1) * ld + D
+    big.raw, big.groups = {}, {"k": None, "v": None}
+    for name in "kv":
+        big.raw[name] = torch.empty(size // 2 if i4 else size, dtype=torch.uint8 if i4 else torch.float16, device=DEV)
+        big.view(big.raw[name], 2 if i4 else 1).copy_(small.view(small.raw[name], 2 if i4 else 1))
+        if i4:
+            big.groups[name] = torch.empty(size // 32, 2, dtype=torch.float16, device=DEV)
+            big.group_view(name).copy_(small.group_view(name))
+    pos = positions([(cap - L, L)], L)
+    q = rnd(1, L, 4, D)
+    check(attend(ns2lib, big, q, pos, 0, 0, True), q, pos, big, 0, 0, True, f"far offsets {L} i4={i4}")
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("L", [1, 90])
+def test_large_scores(ns2lib, L, fp16):
+    """Scores of hundreds, rising and falling along the keys, and scores that are all -inf or equal."""
+    rnd = gen(14)
+    D, cap = 128, 400
+    cache = Cache(rnd, 2, cap, 1, D, False)
+    ramp = torch.linspace(-1, 1, cap, device=DEV)
+    k = torch.zeros(2, cap, 1, D, device=DEV)
+    k[0, :, 0, 0], k[1, :, 0, 0] = ramp, -ramp
+    cache.view(cache.raw["k"], 1).copy_(k.half())
+    cache.value["k"] = k.half().double()
+    q = torch.zeros(2, L, 2, D, device=DEV)
+    q[..., 0, 0], q[..., 1, 0] = 4096.0, 0.0
+    pos = positions([(cap - L, L)] * 2, L)
+    check(attend(ns2lib, cache, q, pos, 0, 0, fp16), q, pos, cache, 0, 0, fp16, f"large scores {L} fp16={fp16}")
+
+
+def test_other_scale_and_repeated_calls(ns2lib):
+    """A scale of one's own; the same call twice gives the same bits (long split sums included)."""
+    rnd = gen(15)
+    cache = Cache(rnd, 2, 3000, 2, 64, True)
+    for L in (1, 100):
+        pos = positions([(2800, L), (1500, L)], L)
+        q = rnd(2, L, 8, 64)
+        a = attend(ns2lib, cache, q, pos, 0, 0, False, scale=0.03)
+        check(a, q, pos, cache, 0, 0, False, f"scale {L}", scale=0.03)
+        assert torch.equal(a, attend(ns2lib, cache, q, pos, 0, 0, False, scale=0.03))
+
+
+# ---- new tokens into a cache -----------------------------------------------------------------------
+
+def write(lib, x, pos, H, KH, D, cap, *, i4, fp16, wq, wk, cs, rope_rows, fill, pad=0):
+    """Returns q rows, and k, v, their groups as [B, cap, KH, ...] buffers that held `fill` before."""
+    B, L = pos.shape
+    ld = KH * D + pad
+    size = B * cap * ld
+    q = torch.full((B * L, H * D + 8), 7.0, dtype=torch.float16 if fp16 else torch.float32, device=DEV)
+    out = {"q": q}
+    for n in "kv":
+        if i4:
+            out[n] = torch.full((size // 2,), int(fill), dtype=torch.uint8, device=DEV)
+            out[n + "g"] = torch.full((size // 32, 2), float(fill), dtype=torch.float16, device=DEV)
+        else:
+            out[n] = torch.full((size,), float(fill), dtype=torch.float16, device=DEV)
+    lib.head_norm_cache(x, pos, q, out["k"], out["v"], batch=B, L=L, H=H, KH=KH, D=D, ldx=x.shape[1], ldq=H * D + 8, cap=cap,
+                        ldkv=ld, kvBatch=cap * ld, w_q=wq, w_k=wk, cs=cs, sin_off=cs.numel() // 2 if cs is not None else 0,
+                        rope_rows=rope_rows, eps=EPS, q_fmt=int(fp16), k_groups=out.get("kg"), v_groups=out.get("vg"))
+    torch.cuda.synchronize()
+    for n in "kv":
+        if i4:
+            out[n] = out[n].reshape(B, cap, -1)[..., : KH * D // 2].reshape(B, cap, KH, D // 2)
+            out[n + "g"] = out[n + "g"].reshape(B, cap, -1, 2)[:, :, : KH * D // 32].reshape(B, cap, KH, D // 32, 2)
+        else:
+            out[n] = out[n].reshape(B, cap, ld)[..., : KH * D].reshape(B, cap, KH, D)
+    return out
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("H,KH,D", HEADS)
+def test_write(ns2lib, H, KH, D, i4, fp16):
+    """Norm, rotation at the position and storage. fp32 arithmetic is off by at most 2^-20 of the head's largest
+    magnitude (a D-term sum of squares in a square root, a few products); fp16 storage by 2^-11 of the value, 4-bit
+    storage by half a step, plus the roundings of the offset (2^-11 |o|) and of the step (2^-11 of 15 steps)."""
+    rnd = gen(H + D)
+    cap, L = 90, 37
+    spans = [(0, L), (50, L - 5), (cap - 3, 3)]
+    pos = positions(spans, L)
+    pos[1, 3] = cap  # past the cache: padding
+    x = rnd(3 * L, (H + 2 * KH) * D + 4) * 3
+    wq, wk = 1 + 0.2 * rnd(D), 1 + 0.2 * rnd(D)
+    for norms, rows in (((wq, wk), cap), ((wq, None), 60), ((None, wk), 0)):
+        cs = R.rope_table(cap, D).to(DEV) if rows else None
+        got = write(ns2lib, x, pos, H, KH, D, cap, i4=i4, fp16=fp16, wq=norms[0], wk=norms[1], cs=cs, rope_rows=rows, fill=9,
+                    pad=32)
+        flat = pos.flatten()
+        live = (flat >= 0) & (flat < cap)
+        heads = x[:, : (H + 2 * KH) * D].double().reshape(3 * L, H + 2 * KH, D)
+        ref = {"q": R.head_norm(heads[:, :H], norms[0], cs, flat, rows, EPS),
+               "k": R.head_norm(heads[:, H: H + KH], norms[1], cs, flat, rows, EPS), "v": heads[:, H + KH:]}
+        q = got["q"]
+        assert (q[:, H * D:] == 7).all() and (q[~live] == 7).all(), "padding of q was written"
+        qv = q[live, : H * D].double().reshape(-1, H, D)
+        qr = ref["q"][live]
+        slack = qr.abs().amax(-1, keepdim=True) * 2.0**-20
+        assert ((qv - qr).abs() <= slack + (2.0**-11 * qr.abs() if fp16 else 0)).all(), "q"
+        b = torch.arange(3, device=DEV).repeat_interleave(L)[live]
+        at = flat[live].long()
+        for n in "kv":
+            r = ref[n][live]
+            slack = r.abs().amax(-1, keepdim=True) * 2.0**-20
+            untouched = torch.ones(3, cap, dtype=torch.bool, device=DEV)
+            untouched[b, at] = False
+            assert (got[n][untouched] == 9).all(), f"other rows of {n} were written"
+            if i4:
+                assert (got[n + "g"][untouched] == 9).all(), f"other groups of {n} were written"
+                groups = got[n + "g"][b, at]
+                step, off = (groups[..., i].double().repeat_interleave(32, -1) for i in (0, 1))
+                val = R.cache_values(got[n][b, at], groups)
+                bound = step / 2 + 2.0**-11 * (off.abs() + 15 * step + val.abs()) + slack
+                assert ((val - r).abs() <= bound).all(), n
+                assert (step <= (r.unflatten(-1, (-1, 32)).amax(-1) - r.unflatten(-1, (-1, 32)).amin(-1)).repeat_interleave(32, -1) / 15
+                        * (1 + 2.0**-10) + slack).all(), f"steps of {n}"
+            else:
+                assert ((got[n][b, at].double() - r).abs() <= 2.0**-11 * r.abs() + slack + 2.0**-24).all(), n
+
+
+def test_four_bit_codes_exactly(ns2lib):
+    """Values that are not normed: codes and groups equal the definition, also for equal values, zeros, tiny and
+    huge ranges and values on a border between two codes."""
+    rnd = gen(21)
+    D, L = 128, 64
+    x = rnd(L, 3 * D)
+    v = x[:, 2 * D:]
+    v[0] = 0.0
+    v[1] = 1.2345
+    v[2] = torch.arange(D, device=DEV) % 32 * 0.5
+    v[3] *= 1e-7
+    v[4] *= 1e4
+    v[5, ::2] = -3.0
+    v[6] = v[6].abs() + 100
+    pos = positions([(0, L)], L)
+    got = write(ns2lib, x, pos, 1, 1, D, L, i4=True, fp16=False, wq=None, wk=None, cs=None, rope_rows=0, fill=1)
+    for n, r in (("k", x[:, D: 2 * D]), ("v", v)):
+        codes, groups = R.cache_codes(r.cpu().reshape(L, 1, D))
+        assert torch.equal(got[n + "g"][0].cpu(), groups), n
+        assert torch.equal(got[n][0].cpu(), codes), n
+
+
+@pytest.mark.parametrize("i4", [False, True])
+def test_values_that_are_not_numbers(ns2lib, i4):
+    """A NaN or an infinity stays visible in its own group (or value) and nowhere else."""
+    rnd = gen(22)
+    D, L = 96, 5
+    x = rnd(L, 3 * D)
+    x[1, 2 * D + 40], x[2, 2 * D + 3], x[3, 2 * D + 95] = math.nan, math.inf, -math.inf
+    got = write(ns2lib, x, positions([(0, L)], L), 1, 1, D, L, i4=i4, fp16=False, wq=None, wk=None, cs=None, rope_rows=0, fill=0)
+    val = (R.cache_values(got["v"], got["vg"]) if i4 else got["v"].double())[0, :, 0]
+    bad = torch.zeros(L, D, dtype=torch.bool, device=DEV)
+    if i4:
+        bad[1, 32:64], bad[2, 0:32], bad[3, 64:96] = True, True, True
+    else:
+        bad[1, 40], bad[2, 3], bad[3, 95] = True, True, True
+    assert torch.equal(~torch.isfinite(val), bad)
+
+
+def test_queries_in_place(ns2lib):
+    """q may be X itself."""
+    rnd = gen(23)
+    H, KH, D, L = 4, 1, 256, 9
+    x = rnd(L, (H + 2 * KH) * D)
+    w = 1 + 0.1 * rnd(D)
+    cs = R.rope_table(L, D).to(DEV)
+    k, v = (torch.zeros(L, D, dtype=torch.float16, device=DEV) for _ in "kv")
+    q = torch.zeros(L, H * D, device=DEV)
+    y = x.clone()
+    for src, dst, ld in ((x, q, H * D), (y, y, x.shape[1])):
+        ns2lib.head_norm_cache(src, positions([(0, L)], L), dst, k, v, batch=1, L=L, H=H, KH=KH, D=D, ldx=x.shape[1], ldq=ld, cap=L,
+                               ldkv=D, kvBatch=L * D, w_q=w, w_k=w, cs=cs, sin_off=cs.numel() // 2, rope_rows=L)
+    torch.cuda.synchronize()
+    assert torch.equal(y[:, : H * D], q) and torch.equal(y[:, H * D:], x[:, H * D:])
+
+
+# ---- graphs, streams, refusals ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("i4", [False, True])
+def test_recorded_steps(ns2lib, i4):
+    """A step (write, then attention) recorded once and replayed for later positions, with eager work and
+    synchronizations between the replays: each replay equals the eager calls on a cache of its own."""
+    rnd = gen(31)
+    B, H, KH, D, cap = 3, 4, 1, 256, 700
+    stream = torch.cuda.Stream()
+    ns2lib.set_stream(stream.cuda_stream)
+    try:
+        with torch.cuda.stream(stream):
+            caches = [Cache(gen(32), B, cap, KH, D, i4) for _ in range(2)]
+            x = rnd(B, (H + 2 * KH) * D)
+            pos = torch.tensor([[600], [20], [-1]], dtype=torch.int32, device=DEV)
+            w = 1 + 0.1 * rnd(D)
+            cs = R.rope_table(cap, D).to(DEV)
+            need = ns2lib.attention_cache_bytes(B, 1, H, KH, D, cap, 512, 4)
+            bufs = [(torch.zeros(B, H * D, dtype=torch.float16, device=DEV), torch.zeros(B, H * D, dtype=torch.float16, device=DEV),
+                     torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)) for _ in range(2)]
+
+            def step(i):
+                q, o, work = bufs[i]
+                c = caches[i]
+                ns2lib.head_norm_cache(x, pos, q, c.raw["k"], c.raw["v"], L=1, H=H, ldx=x.shape[1], ldq=H * D, w_q=w, w_k=w, cs=cs,
+                                       sin_off=cs.numel() // 2, rope_rows=cap, q_fmt=1, **c.args())
+                ns2lib.attention_cache(q, pos, c.raw["k"], c.raw["v"], o, L=1, H=H, ldq=H * D, ldo=H * D, window=512, sinks=4, q_fmt=1,
+                                       work=work, **c.args())
+
+            stream.synchronize()
+            ns2lib.graph_begin()
+            step(0)
+            graph = ns2lib.graph_end()
+            for n in range(5):
+                x.copy_(rnd(*x.shape))
+                ns2lib.graph_launch(graph)
+                step(1)
+                stream.synchronize()
+                assert torch.equal(bufs[0][1], bufs[1][1]), f"replay {n}"
+                for name in "kv":
+                    assert torch.equal(caches[0].raw[name], caches[1].raw[name])
+                pos += (pos >= 0).int()
+                _ = torch.randn(1000, 1000, device=DEV).sum().item()
+            ns2lib.graph_destroy(graph)
+            assert (bufs[0][1][2] == 0).all()
+    finally:
+        ns2lib.set_stream(torch.cuda.current_stream().cuda_stream)
+
+
+BASE = dict(batch=1, L=1, H=4, KH=2, D=64, cap=64, ldkv=128, kvBatch=64 * 128, ldq=256)
+
+
+@pytest.mark.parametrize("change", [dict(D=80), dict(D=32), dict(D=512), dict(H=3), dict(KH=0), dict(H=0), dict(cap=0), dict(ldq=255),
+                                    dict(ldq=258), dict(ldkv=120), dict(ldkv=132), dict(kvBatch=-8), dict(kvBatch=8196), dict(q_fmt=2),
+                                    dict(window=-1), dict(sinks=-1), dict(ldo=128), dict(ldo=257), dict(k=None), dict(v=None),
+                                    dict(pos=None), dict(q=None), dict(o=None), dict(vg=None), dict(k=8), dict(q=4), dict(o=4)])
+def test_attention_refusals(ns2lib, change):
+    """Refused on the host, before any launch: the output keeps what it held."""
+    import ns2
+
+    t = {n: torch.zeros(64 * 128, device=DEV) for n in ("q", "k", "v", "o", "kg", "vg")}
+    t["pos"] = torch.zeros(1, dtype=torch.int32, device=DEV)
+    a = dict(BASE, ldo=256, window=0, sinks=0, q_fmt=0, kg=None, vg=None)
+    ptr = {n: t[n] for n in ("q", "pos", "k", "v", "o")}
+    if "vg" in change:
+        a["kg"] = t["kg"]
+    for n, x in change.items():
+        if n in ptr:
+            ptr[n] = None if x is None else ptr[n].data_ptr() + x
+        else:
+            a[n] = x
+    kg, vg = a.pop("kg"), a.pop("vg")
+    need = ns2lib.attention_cache_bytes(1, 1, 4, 2, 64, 64, 0, 0)
+    work = torch.zeros(max(need, 16), dtype=torch.uint8, device=DEV)
+    with pytest.raises(ns2.NS2Error, match="ns2_attention_cache"):
+        ns2lib.attention_cache(ptr["q"], ptr["pos"], ptr["k"], ptr["v"], ptr["o"], k_groups=kg, v_groups=vg, work=work, **a)
+    torch.cuda.synchronize()
+    assert (t["o"] == 0).all()
+
+
+@pytest.mark.parametrize("change", [dict(D=48), dict(H=5), dict(ldx=500), dict(ldx=514), dict(x=4), dict(x=None), dict(wk=4), dict(cs=4),
+                                    dict(sin_off=2), dict(sin_off=-4), dict(rope_rows=-1), dict(batch=2, kvBatch=64), dict(kvBatch=8196),
+                                    dict(kg=None), dict(k=2), dict(ldq=250)])
+def test_write_refusals(ns2lib, change):
+    import ns2
+
+    t = {n: torch.zeros(128 * 128, device=DEV) for n in ("x", "q", "k", "v", "kg", "vg", "wk", "cs")}
+    t["pos"] = torch.zeros(2, dtype=torch.int32, device=DEV)
+    a = dict(BASE, ldx=512, sin_off=64, rope_rows=2, q_fmt=0)
+    ptr = {n: t[n] for n in ("x", "pos", "q", "k", "v", "wk", "cs", "kg", "vg")}
+    if not set(change) & {"kg"}:
+        ptr["kg"] = ptr["vg"] = None
+    for n, x in change.items():
+        if n in ptr:
+            ptr[n] = None if x is None else ptr[n].data_ptr() + x
+        else:
+            a[n] = x
+    with pytest.raises(ns2.NS2Error, match="ns2_head_norm_cache"):
+        ns2lib.head_norm_cache(ptr["x"], ptr["pos"], ptr["q"], ptr["k"], ptr["v"], w_k=ptr["wk"], cs=ptr["cs"], k_groups=ptr["kg"],
+                               v_groups=ptr["vg"], **a)
+    torch.cuda.synchronize()
+    assert (t["q"] == 0).all() and (t["k"] == 0).all()
+
+
+def test_work_memory_is_checked(ns2lib):
+    """Too little work memory, or none where some is needed, is refused; nothing to do is no error."""
+    import ns2
+
+    a = dict(batch=1, L=1, H=4, KH=1, D=256, cap=65536, ldkv=256, kvBatch=65536 * 256)
+    need = ns2lib.attention_cache_bytes(1, 1, 4, 1, 256, 65536, 0, 0)
+    q, o, kv = torch.zeros(1024, device=DEV), torch.zeros(1024, device=DEV), torch.zeros(65536 * 256, dtype=torch.float16, device=DEV)
+    pos = torch.zeros(1, dtype=torch.int32, device=DEV)
+    if need:
+        for work in (None, torch.empty(need - 16, dtype=torch.uint8, device=DEV)):
+            with pytest.raises(ns2.NS2Error, match="work memory"):
+                ns2lib.attention_cache(q, pos, kv, kv, o, ldq=1024, ldo=1024, work=work, **a)
+    a["batch"] = 0
+    ns2lib.attention_cache(q, pos, kv, kv, o, ldq=1024, ldo=1024, **a)
+    a.update(batch=1, L=0)
+    ns2lib.attention_cache(q, pos, kv, kv, o, ldq=1024, ldo=1024, **a)
