@@ -292,8 +292,8 @@ int ns2_attention_rows_f16kv_oproj(const float* q, const uint16_t* k, const uint
  *   j < sinks or j > p - window (window = 0: all j <= p).
  * What the cache holds at other positions, infinities and NaN too, does not matter. kvBatch = 0 lets
  * all sequences read one cache. fp16 q: the softmax weights are rounded to fp16 for the second
- * product; fp32 q: queries and weights take part as sums of fp16 parts that keep 22 of their bits
- * (a query times `scale` must lie in fp16's range). Sums and softmax statistics are fp32. work:
+ * product; fp32 q: queries and weights take part as sums of fp16 parts that keep 22 of their bits.
+ * Sums and softmax statistics are fp32; the same call gives the same bits again. work:
  * ns2_attention_cache_bytes bytes of device memory that the call may write (NULL where that is 0);
  * calls that may overlap take one each. */
 int ns2_head_norm_cache(const float* X, int ldx, const int* pos, const float* w_q, const float* w_k,

@@ -1,0 +1,290 @@
+// Shared by the cache kernels (ns2_cache.hip, ns2_cache_rows.hip, ns2_cache_prompt.hip): the layout of a
+// cache, its 4-bit values, which keys a tile of query columns sees, and the softmax's running state.
+//
+// Attention runs transposed: S^T = K Q^T and O^T = V^T P^T, both with v_mfma_f32_16x16x32_f16. A product's
+// result holds one query per lane column (lane % 16) and four rows per lane (4 (lane / 16) + r), so that
+// the weights p of two 16-key score tiles are, in place, the B operand of the second product: operand
+// element j of lane group grp is key 4 grp + j of the first tile (j < 4) or of the second (j >= 4). V^T's
+// operand takes its keys in the same order. A "column" is one (token, query head) pair of a K/V head, token
+// by token, so that the heads of a group share every key that is loaded.
+#pragma once
+
+#include <type_traits>
+
+#include "ns2_common.h"
+
+namespace ns2cache {
+
+using namespace ns2dev;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kGroup = 32;  // values per step and offset of a 4-bit cache
+
+struct AttnArgs {
+  const void* q;
+  const int* pos;
+  const void *k, *v;
+  const half2_t *kg, *vg;  // (step, offset) of a 4-bit cache
+  void* o;
+  float* part_o;   // splits > 1: [splits][batch*KH][R][D] sums over a split's keys
+  float2* part_s;  // and their (maximum, sum of weights)
+  long long kvBatch;
+  int ldq, ldo, ldkv, L, H, KH, cap, window, sinks, q_fmt, batch, splits;
+  float scale;  // times log2(e)
+};
+
+struct Plan {
+  bool prompt;  // ns2_cache_prompt.hip, else ns2_cache_rows.hip
+  int splits;
+};
+
+int launch_rows(const AttnArgs& a, int D, hipStream_t s);
+int launch_prompt(const AttnArgs& a, int D, hipStream_t s);
+
+// ---- 4-bit values ----------------------------------------------------------------------------
+
+// Four nibbles of each 16-bit half of x -> the half2 pairs (n0, n0'), (n1, n1') ...: 0x6400 | n is the half
+// 1024 + n, the subtraction is exact, and the fused multiply-add rounds offset + n * step once.
+__device__ __forceinline__ void dequant4(uint32_t x, half2_t s, half2_t o, uint32_t r[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const half2_t n = __builtin_bit_cast(half2_t, ((x >> (4 * i)) & 0x000f000fu) | 0x64006400u) - half2_t{1024.f, 1024.f};
+    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, s, o));
+  }
+}
+
+// A word's eight values in the order 0 4 1 5 2 6 3 7 (operand elements; Q's are put in the same order).
+__device__ __forceinline__ half8_t dequant8(uint32_t w, half2_t so) {
+  uint32_t r[4];
+  dequant4(w, half2_t{so[0], so[0]}, half2_t{so[1], so[1]}, r);
+  return __builtin_bit_cast(half8_t, make_uint4(r[0], r[1], r[2], r[3]));
+}
+
+// (low half of a, low half of b) and (high half of a, high half of b)
+__device__ __forceinline__ uint32_t pair_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ uint32_t pair_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// ---- columns and the keys they see --------------------------------------------------------------
+
+template <int CTRL>
+__device__ __forceinline__ int dpp_i(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, false);
+}
+__device__ __forceinline__ int row16_max(int v) {
+  v = max(v, dpp_i<kDppXor1>(v));
+  v = max(v, dpp_i<kDppXor2>(v));
+  v = max(v, dpp_i<kDppHalfMirror>(v));
+  return max(v, dpp_i<kDppRowMirror>(v));
+}
+// Maximum over the four lanes that hold one column (lane % 16).
+__device__ __forceinline__ float column_max(float v) {
+  float a = v, b = v;
+  permlane16_swap(a, b);
+  a = fmaxf(a, b);
+  b = a;
+  permlane32_swap(a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float column_sum(float v) {
+  float a = v, b = v;
+  permlane16_swap(a, b);
+  a = a + b;
+  b = a;
+  permlane32_swap(a, b);
+  return a + b;
+}
+
+// Position of column m (-1: padding, or past the last column).
+__device__ __forceinline__ int column_pos(const AttnArgs& a, int b, int m) {
+  const int G = a.H / a.KH;
+  if (m >= a.L * G) return -1;
+  const int p = a.pos[(long long)b * a.L + m / G];
+  return p < a.cap ? p : -1;
+}
+
+// The keys that some column of a block sees, as tiles of KT: the first tokens [0, first) that are outside
+// every window, then [lo, last].
+struct Keys {
+  int pmin, pmax, lo, first, tiles_first, tiles;
+};
+
+template <int KT>
+__device__ __forceinline__ Keys keys_of(const AttnArgs& a, int pmin, int pmax) {
+  Keys k;
+  k.pmin = pmin;
+  k.pmax = pmax;
+  k.lo = a.window && pmin >= a.window ? pmin - a.window + 1 : 0;
+  k.first = a.sinks < k.lo ? a.sinks : k.lo;
+  k.tiles_first = (k.first + KT - 1) / KT;
+  k.tiles = k.tiles_first + (pmax - k.lo) / KT + 1;
+  return k;
+}
+
+struct Tile {
+  int key0, end;  // keys [key0, end) of the tile exist; loads past them repeat the last one
+  bool whole;     // every column sees every key
+};
+
+template <int KT>
+__device__ __forceinline__ Tile tile_of(const AttnArgs& a, const Keys& k, int t) {
+  Tile r;
+  const bool first = t < k.tiles_first;
+  r.key0 = first ? t * KT : k.lo + (t - k.tiles_first) * KT;
+  r.end = first ? k.first : k.pmax + 1;
+  const int last = r.key0 + KT - 1;
+  r.whole = last < r.end && last <= k.pmin && (!a.window || r.key0 > k.pmax - a.window || last < a.sinks);
+  return r;
+}
+
+__device__ __forceinline__ bool sees(const AttnArgs& a, int p, int key, int end) {
+  return key < end && key <= p && (!a.window || key > p - a.window || key < a.sinks);
+}
+
+// ---- queries -------------------------------------------------------------------------------------
+
+// Element e of operand step t of lane group grp is dimension qdim(t, grp) + e (fp16 cache: e in order, 4-bit:
+// in the order of dequant8). A lane's K values are 8 apart from its neighbours' in an fp16 row, and one
+// contiguous quarter of a 4-bit row.
+template <int D, bool I4>
+__device__ __forceinline__ int qdim(int t, int grp) {
+  return I4 ? grp * (D / 4) + 8 * t : 32 * t + 8 * grp;
+}
+
+// Column m's query, or null for padding (whose operands are zeros).
+template <bool F32>
+struct Query {
+  const char* at;
+  int up;      // fp32: scaled by 2^up, to below 2^14
+  float mult;  // what takes a score to a base-2 logarithm
+
+  __device__ __forceinline__ float4 four(int d) const {
+    return at ? *reinterpret_cast<const float4*>(at + 4 * d) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  template <int D, bool I4>
+  __device__ __forceinline__ void open(const AttnArgs& a, int b, int g, int m, bool live, int grp) {
+    const int G = a.H / a.KH, i = live ? m / G : 0, h = live ? m - i * G : 0;
+    const long long e = ((long long)b * a.L + i) * a.ldq + (long long)(g * G + h) * D;
+    at = live ? static_cast<const char*>(a.q) + e * (F32 ? 4 : 2) : nullptr;
+    mult = a.scale;
+    up = 0;
+    if constexpr (F32) {
+      float top = 0.f;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) {
+        const float4 u = four(qdim<D, I4>(t, grp)), v = four(qdim<D, I4>(t, grp) + 4);
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))));
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+      }
+      top = column_max(top);
+      if (top > 0.f && top < INFINITY) up = min(14 - __builtin_amdgcn_frexp_expf(top), 120);
+      mult = ldexpf(a.scale, -up);
+    }
+  }
+  // The B operand of step t; PERM: in the order of dequant8. fp32: two halves that keep 22 bits.
+  template <int D, bool I4, bool PERM>
+  __device__ __forceinline__ void operand(int t, int grp, half8_t& hi, half8_t& lo) const {
+    constexpr int order[8] = {0, PERM ? 4 : 1, PERM ? 1 : 2, PERM ? 5 : 3, PERM ? 2 : 4, PERM ? 6 : 5, PERM ? 3 : 6, 7};
+    const int d = qdim<D, I4>(t, grp);
+    if constexpr (!F32) {
+      const half8_t x = at ? *reinterpret_cast<const half8_t*>(at + 2 * d) : half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) hi[e] = x[order[e]];
+    } else {
+      const float4 u = four(d), v = four(d + 4);
+      const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = ldexpf(x[order[e]], up);
+        hi[e] = (half_t)y;
+        lo[e] = (half_t)(y - (float)hi[e]);
+      }
+    }
+  }
+};
+
+// ---- the softmax's running state -------------------------------------------------------------------
+
+// The reference m of a column trails its maximum by up to 2^kSlack: only a score above m + kSlack moves it
+// and rescales the sums, so that most tiles leave the accumulators alone. Weights are then at most 2^kSlack.
+constexpr float kSlack = 8.f;
+
+// Scores s[N] (base-2 logarithms, -inf where masked) of the lane's column -> weights in place; returns
+// whether the lane's column moved its reference, with the factor for what was summed before.
+template <int N>
+__device__ __forceinline__ bool soften(float (&s)[N], float& m, float& l, float& corr) {
+  float top = s[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, s[i]);
+  top = column_max(top);
+  const bool moves = top > m + kSlack;
+  corr = 1.f;
+  if (moves) {
+    corr = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    m = top;
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+    sum += s[i];
+  }
+  l = l * corr + sum;
+  return moves;
+}
+
+__device__ __forceinline__ float4_t mfma(half8_t a, half8_t b, float4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// The B operand of the second product: eight weights, as halves hi (+ lo).
+template <bool F32>
+__device__ __forceinline__ void weights(const float* p, half8_t& hi, half8_t& lo) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    hi[e] = (half_t)p[e];
+    if constexpr (F32) lo[e] = (half_t)(p[e] - (float)hi[e]);
+  }
+}
+
+// Values that are not finite must reach the columns that see them and no others, but 0 * inf is NaN: they are
+// taken out of the product, and a second product of marks (1 for inf, 64 for -inf, 4096 for NaN) with the
+// columns' visible keys (1 or 0) tells each output what it has seen (at most 32 of each per product).
+__device__ __forceinline__ half8_t without_marked(half8_t v, half8_t& mark) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const half_t x = v[e];  // (a bit cast of the element itself would read element 0)
+    const uint16_t u = __builtin_bit_cast(uint16_t, x), size = u & 0x7fffu;
+    mark[e] = size < 0x7c00u ? (half_t)0.f : size > 0x7c00u ? (half_t)4096.f : u == size ? (half_t)1.f : (half_t)64.f;
+    v[e] = size < 0x7c00u ? x : (half_t)0.f;
+  }
+  return v;
+}
+__device__ __forceinline__ float4_t with_seen(float4_t o, float4_t count) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = (int)count[i], plus = c & 63, minus = (c >> 6) & 63;
+    if (c) o[i] += c >= 4096 || (plus && minus) ? NAN : plus ? INFINITY : -INFINITY;
+  }
+  return o;
+}
+
+// Adds 0 * v: NaN once v held an infinity or a NaN.
+__device__ __forceinline__ void spot(half8_t v, half2_t& z) {
+  const uint4 w = __builtin_bit_cast(uint4, v);
+  const half2_t zero = {0.f, 0.f};
+  z = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, w.x), zero, z);
+  z = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, w.y), zero, z);
+  z = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, w.z), zero, z);
+  z = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, w.w), zero, z);
+}
+
+}  // namespace ns2cache
+
+#define NS2_CACHE_D(D, LAUNCH)  \
+  switch (D) {                  \
+    case 64: LAUNCH(64) break;   \
+    case 96: LAUNCH(96) break;   \
+    case 128: LAUNCH(128) break; \
+    default: LAUNCH(256) break;  \
+  }

@@ -6,14 +6,13 @@
 // b*kvBatch + j*ldkv + g*D. An fp16 cache holds them as they are. A 4-bit cache holds codes c two
 // to a byte (the even value in the low four bits) and, per 32 values, an fp16 step s and offset o;
 // it stands for the fp16 values half(o + c*s).
-#include "ns2_common.h"
+#include <algorithm>
 
-using namespace ns2dev;
+#include "ns2_cache.h"
+
+using namespace ns2cache;
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kGroup = 32;  // values per step and offset of a 4-bit cache
 
 inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
@@ -128,106 +127,60 @@ __global__ __launch_bounds__(256) void cache_write_kernel(WriteArgs a) {
   }
 }
 
-// ---- attention over the cache --------------------------------------------------------------------
+// ---- attention: the splits joined, and which kernel runs ---------------------------------------------
 
-struct CacheAttnArgs {
-  const void* q;
-  const int* pos;
-  const void *k, *v;
-  const half2_t *kg, *vg;
-  void* o;
-  long long kvBatch, rows;
-  int ldq, ldo, ldkv, L, H, KH, cap, window, sinks, q_fmt;
-  float scale;  // times log2(e)
-};
-
-// 8 cached values from value index `at` (a multiple of 8)
-template <bool I4>
-__device__ __forceinline__ half8_t cached8(const void* c, const half2_t* g, long long at) {
-  if constexpr (!I4) {
-    return *reinterpret_cast<const half8_t*>(static_cast<const half_t*>(c) + at);
-  } else {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c) + at / 2);
-    const half2_t so = g[at / kGroup];
-    half8_t r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = __builtin_fmaf16((half_t)(float)((w >> (4 * i)) & 15), so[0], so[1]);
-    return r;
+// One wave per column: the splits' sums weighted to their common maximum, in split order. A split that saw no
+// key has maximum -inf and its sums are not read.
+__global__ __launch_bounds__(256) void cache_join_kernel(AttnArgs a, int D) {
+  const int lane = threadIdx.x & 63;
+  const int G = a.H / a.KH, R = a.L * G;
+  const long long columns = (long long)a.batch * a.KH * R, u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (u >= columns) return;
+  const int bg = (int)(u / R), mc = (int)(u - (long long)bg * R), b = bg / a.KH, g = bg - b * a.KH;
+  if (column_pos(a, b, mc) < 0) return;
+  float top = -INFINITY;
+  for (int z = 0; z < a.splits; ++z) top = fmaxf(top, a.part_s[z * columns + u].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, r[4] = {0.f, 0.f, 0.f, 0.f};
+  const int d = 4 * lane;
+  for (int z = 0; z < a.splits; ++z) {
+    const float2 ml = a.part_s[z * columns + u];
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
+    sum += f * ml.y;
+    if (d < D) {
+      const float4 x = *reinterpret_cast<const float4*>(a.part_o + (z * columns + u) * D + d);
+      r[0] += f * x.x;
+      r[1] += f * x.y;
+      r[2] += f * x.z;
+      r[3] += f * x.w;
+    }
   }
+  if (d >= D) return;
+  const float inv = 1.f / sum;
+  const int i = mc / G;
+  const long long at = ((long long)b * a.L + i) * a.ldo + (long long)(g * G + mc - i * G) * D + d;
+  if (a.q_fmt)
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack_half2(r[0] * inv, r[1] * inv), pack_half2(r[2] * inv, r[3] * inv));
+  else
+    *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = make_float4(r[0] * inv, r[1] * inv, r[2] * inv, r[3] * inv);
 }
 
-// One wave per (token, query head): 64 visible keys at a time, a key per lane for the scores and
-// D / 64 output values per lane for the sum.
-template <int D, bool I4>
-__global__ __launch_bounds__(256) void cache_attn_kernel(CacheAttnArgs a) {
-  constexpr int DL = (D + 63) / 64;
-  __shared__ float q_s[4][D];
-  __shared__ float p_s[4][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long long u = (long long)blockIdx.x * 4 + wave;
-  if (u >= a.rows * a.H) return;
-  const long long row = u / a.H;
-  const int h = (int)(u - row * a.H), g = h / (a.H / a.KH);
-  const int p = a.pos[row];
-  if (p < 0 || p >= a.cap) return;
-  for (int d = lane; d < D; d += 64) {
-    const long long at = row * a.ldq + (long long)h * D + d;
-    q_s[wave][d] = a.q_fmt ? (float)static_cast<const half_t*>(a.q)[at] : static_cast<const float*>(a.q)[at];
-  }
-  const int lo = a.window && p >= a.window ? p - a.window + 1 : 0;
-  const int first = a.sinks < lo ? a.sinks : lo;
-  const int n = first + p - lo + 1;
-  const long long base = (row / a.L) * a.kvBatch + (long long)g * D;
-  float m = -INFINITY, l = 0.f, o[DL];
-#pragma unroll
-  for (int i = 0; i < DL; ++i) o[i] = 0.f;
-  for (int t0 = 0; t0 < n; t0 += 64) {
-    const int cnt = n - t0 < 64 ? n - t0 : 64;
-    const int t = t0 + (lane < cnt ? lane : 0);
-    const int key = t < first ? t : lo + t - first;
-    float s = 0.f;
-    for (int d = 0; d < D; d += 8) {
-      const half8_t k8 = cached8<I4>(a.k, a.kg, base + (long long)key * a.ldkv + d);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s = fmaf((float)k8[i], q_s[wave][d + i], s);
-    }
-    s = lane < cnt ? s * a.scale : -INFINITY;
-    float mx = s;
-    for (int i = 1; i < 64; i <<= 1) mx = fmaxf(mx, __shfl_xor(mx, i));
-    const float mn = fmaxf(m, mx);
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    const float corr = exp2f(m - ref);
-    const float e = exp2f(s - ref);
-    l = l * corr + wave_sum(e);
-    m = mn;
-    __builtin_amdgcn_wave_barrier();
-    p_s[wave][lane] = e;
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int i = 0; i < DL; ++i) o[i] *= corr;
-    for (int c = 0; c < cnt; ++c) {
-      const int tc = t0 + c;
-      const long long at = base + (long long)(tc < first ? tc : lo + tc - first) * a.ldkv;
-      const float e = p_s[wave][c];
-#pragma unroll
-      for (int i = 0; i < DL; ++i) {
-        const int d = lane + 64 * i;
-        if (d < D) {
-          const half8_t v8 = cached8<I4>(a.v, a.vg, at + (d & ~7));
-          o[i] = fmaf(e, (float)v8[d & 7], o[i]);
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < DL; ++i) {
-    const int d = lane + 64 * i;
-    if (d < D) {
-      const long long at = row * a.ldo + (long long)h * D + d;
-      if (a.q_fmt) static_cast<half_t*>(a.o)[at] = (half_t)(o[i] / l);
-      else static_cast<float*>(a.o)[at] = o[i] / l;
-    }
-  }
+constexpr int kRowsColumns = 64;  // columns of a K/V head up to which its keys are streamed past 16 at a time
+constexpr long long kCUs = 256;
+
+Plan plan_of(int batch, int L, int H, int KH, int cap, int window, int sinks) {
+  const long long R = (long long)L * (H / KH), heads = (long long)batch * KH;
+  // keys that a block may have to read
+  const long long keys = window ? std::min<long long>(cap, (long long)window + sinks + L) : cap;
+  Plan p;
+  p.prompt = R > kRowsColumns;
+  const long long blocks = heads * (p.prompt ? (R + 63) / 64 : (R + 15) / 16);
+  const long long want = p.prompt ? kCUs / blocks : 2 * kCUs / blocks;
+  // at least four tiles of 64 keys, or two of 32 for each of four waves, per split
+  const long long most = std::max<long long>(1, keys / 256);
+  p.splits = (int)std::max<long long>(1, std::min(want, most));
+  return p;
 }
 
 // The argument checks that both entry points share.
@@ -248,14 +201,6 @@ int check_cache(const char* fn, const void* q, const int* pos, const void* k, co
 }
 
 }  // namespace
-
-#define NS2_CACHE_D(D, LAUNCH)            \
-  switch (D) {                            \
-    case 64: LAUNCH(64) break;            \
-    case 96: LAUNCH(96) break;            \
-    case 128: LAUNCH(128) break;          \
-    default: LAUNCH(256) break;           \
-  }
 
 extern "C" {
 
@@ -291,7 +236,11 @@ int ns2_head_norm_cache(const float* X, int ldx, const int* pos, const float* w_
   return NS2_OK;
 }
 
-size_t ns2_attention_cache_bytes(int batch, int L, int H, int KH, int D, int cap, int window, int sinks) { return 0; }
+size_t ns2_attention_cache_bytes(int batch, int L, int H, int KH, int D, int cap, int window, int sinks) {
+  if (batch <= 0 || L <= 0 || H <= 0 || KH <= 0 || H % KH || D <= 0 || cap <= 0 || window < 0 || sinks < 0) return 0;
+  const int splits = plan_of(batch, L, H, KH, cap, window, sinks).splits;
+  return splits > 1 ? (size_t)splits * batch * L * H * (D + 2) * sizeof(float) : 0;
+}
 
 int ns2_attention_cache(const void* q, int q_fmt, int ldq, const int* pos, const void* k, const void* v, const uint16_t* k_groups,
                         const uint16_t* v_groups, void* o, int ldo, int batch, int L, int H, int KH, int D, int cap, int ldkv,
@@ -306,19 +255,42 @@ int ns2_attention_cache(const void* q, int q_fmt, int ldq, const int* pos, const
   const size_t need = ns2_attention_cache_bytes(batch, L, H, KH, D, cap, window, sinks);
   NS2_REQUIRE(work_bytes >= need && (!need || (work && aligned(work, 16))),
               "%s: the call needs %zu bytes of 16-byte aligned work memory (ns2_attention_cache_bytes), got %zu", fn, need, work_bytes);
-  CacheAttnArgs a{q, pos, k, v, reinterpret_cast<const half2_t*>(k_groups), reinterpret_cast<const half2_t*>(v_groups), o, kvBatch,
-                  (long long)batch * L, ldq, ldo, ldkv, L, H, KH, cap, window, sinks, q_fmt, scale * kLog2e};
-  const long long units = a.rows * H;
-  NS2_REQUIRE((units + 3) / 4 <= INT32_MAX, "%s: %lld query heads are too many for one launch", fn, units);
-  const unsigned grid = (unsigned)((units + 3) / 4);
+  NS2_REQUIRE((long long)L * (H / KH) <= INT32_MAX - 256 && (long long)batch * KH * 64 <= INT32_MAX,
+              "%s: batch=%d, L=%d, H=%d are too many for one launch", fn, batch, L, H);
+  const Plan plan = plan_of(batch, L, H, KH, cap, window, sinks);
+  NS2_REQUIRE((long long)L * (H / KH) <= 64LL * 65535, "%s: L=%d is too many tokens for one launch", fn, L);
+  AttnArgs a{};
+  a.q = q;
+  a.pos = pos;
+  a.k = k;
+  a.v = v;
+  a.kg = reinterpret_cast<const half2_t*>(k_groups);
+  a.vg = reinterpret_cast<const half2_t*>(v_groups);
+  a.o = o;
+  a.part_o = static_cast<float*>(work);
+  if (plan.splits > 1) a.part_s = reinterpret_cast<float2*>(a.part_o + (size_t)plan.splits * batch * L * H * D);
+  a.kvBatch = kvBatch;
+  a.ldq = ldq;
+  a.ldo = ldo;
+  a.ldkv = ldkv;
+  a.L = L;
+  a.H = H;
+  a.KH = KH;
+  a.cap = cap;
+  a.window = window;
+  a.sinks = sinks;
+  a.q_fmt = q_fmt;
+  a.batch = batch;
+  a.splits = plan.splits;
+  a.scale = scale * kLog2e;
   hipStream_t s = ns2::stream();
-  ns2::ProfScope prof_("attention_cache");
-#define NS2_ATTN(D_)                                                        \
-  if (k_groups) cache_attn_kernel<D_, true><<<grid, 256, 0, s>>>(a);        \
-  else cache_attn_kernel<D_, false><<<grid, 256, 0, s>>>(a);
-  NS2_CACHE_D(D, NS2_ATTN)
-#undef NS2_ATTN
-  NS2_LAUNCHED("attention_cache");
+  ns2::ProfScope prof_(plan.prompt ? "attention_cache_prompt" : "attention_cache_rows");
+  if (int rc = plan.prompt ? launch_prompt(a, D, s) : launch_rows(a, D, s)) return rc;
+  if (plan.splits > 1) {
+    const long long columns = (long long)batch * L * H;
+    cache_join_kernel<<<(unsigned)((columns + 3) / 4), 256, 0, s>>>(a, D);
+    NS2_LAUNCHED("cache_join");
+  }
   return NS2_OK;
 }
 

@@ -1,0 +1,344 @@
+// Attention of few query columns over a cache: single tokens, and short runs of them.
+//
+// The cache is read once and that bounds it: 2 D values per key and K/V head for at most 16 columns. A block
+// takes 16 columns of one K/V head and one split of their keys; its four waves take tiles of 32 keys in
+// turn, straight from memory into operand registers, each with a softmax state and accumulators of its own,
+// and merge them through LDS at the end. A tile's next K rows are requested as soon as the scores have used
+// the last ones, its next V rows after the second product, so that a wave always has loads in flight.
+#include "ns2_cache.h"
+
+using namespace ns2cache;
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kTile = 32;  // keys
+
+// The K operands of a tile: rows key0 + 16 s + lane % 16 of step t.
+template <int D, bool I4>
+struct KTile {
+  half8_t x[2][D / 32];
+  __device__ __forceinline__ void load(const AttnArgs& a, long long base, const Tile& t, int col, int grp) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int key = t.key0 + 16 * s + col;
+      const half_t* row = static_cast<const half_t*>(a.k) + base + (long long)(key < t.end ? key : t.end - 1) * a.ldkv;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) x[s][i] = *reinterpret_cast<const half8_t*>(row + qdim<D, false>(i, grp));
+    }
+  }
+  __device__ __forceinline__ half8_t operand(int s, int t, int) const { return x[s][t]; }
+};
+
+template <int D>
+struct KTile<D, true> {
+  static constexpr int W = D / 32, NG = D == 96 ? 3 : D == 256 ? 2 : 1;  // words and groups of a lane's D / 4 values
+  uint32_t w[2][W];
+  half2_t so[2][NG];
+  __device__ __forceinline__ void load(const AttnArgs& a, long long base, const Tile& t, int col, int grp) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int key = t.key0 + 16 * s + col;
+      const long long at = base + (long long)(key < t.end ? key : t.end - 1) * a.ldkv;
+      const uint8_t* row = static_cast<const uint8_t*>(a.k) + at / 2 + grp * (D / 8);
+      if constexpr (D == 96) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[s][i] = reinterpret_cast<const uint32_t*>(row)[i];
+      } else if constexpr (D == 64) {
+        const uint2 x = *reinterpret_cast<const uint2*>(row);
+        w[s][0] = x.x;
+        w[s][1] = x.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(row + 4 * i);
+          w[s][i] = x.x;
+          w[s][i + 1] = x.y;
+          w[s][i + 2] = x.z;
+          w[s][i + 3] = x.w;
+        }
+      }
+      const half2_t* gr = a.kg + at / kGroup;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) so[s][i] = gr[(grp * (D / 4) + (D == 96 ? 8 : 32) * i) / kGroup];
+    }
+  }
+  __device__ __forceinline__ half8_t operand(int s, int t, int) const { return dequant8(w[s][t], so[s][D == 96 ? t : t / 4]); }
+};
+
+// The V^T operands of a tile: lane column c holds dimensions vdim(t, c) of eight keys, a contiguous piece of
+// each row, so that 16 lanes read a row; two keys' halves are paired in registers.
+template <int D, bool I4>
+__device__ __forceinline__ int vdim(int t, int c) {
+  return I4 && D == 96 ? (t < 4 ? 4 * c + t : 64 + 2 * c + t - 4) : D / 16 * c + t;
+}
+
+template <int D, bool I4>
+struct VTile {
+  static constexpr int DT = D / 16;
+  uint32_t x[8][DT / 2];
+  __device__ __forceinline__ void load(const AttnArgs& a, long long base, const Tile& t, int col, int grp) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int key = t.key0 + 4 * grp + (j < 4 ? j : 12 + j);
+      const half_t* row = static_cast<const half_t*>(a.v) + base + (long long)(key < t.end ? key : t.end - 1) * a.ldkv + DT * col;
+      if constexpr (DT % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < DT / 2; i += 4) {
+          const uint4 y = *reinterpret_cast<const uint4*>(row + 2 * i);
+          x[j][i] = y.x;
+          x[j][i + 1] = y.y;
+          x[j][i + 2] = y.z;
+          x[j][i + 3] = y.w;
+        }
+      } else if constexpr (DT == 4) {
+        const uint2 y = *reinterpret_cast<const uint2*>(row);
+        x[j][0] = y.x;
+        x[j][1] = y.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < DT / 2; ++i) x[j][i] = reinterpret_cast<const uint32_t*>(row)[i];
+      }
+    }
+  }
+  // makes the next each() start from the loaded values again, instead of keeping every operand of the last
+  __device__ __forceinline__ void again() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int i = 0; i < DT / 2; ++i) asm volatile("" : "+v"(x[j][i]));
+  }
+  // calls f(t, operand) for every step of 16 dimensions
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      uint32_t r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = t & 1 ? pair_hi(x[2 * i][t / 2], x[2 * i + 1][t / 2]) : pair_lo(x[2 * i][t / 2], x[2 * i + 1][t / 2]);
+      f(t, __builtin_bit_cast(half8_t, make_uint4(r[0], r[1], r[2], r[3])));
+    }
+  }
+};
+
+template <int D>
+struct VTile<D, true> {
+  static constexpr int DT = D / 16, W = D == 256 ? 2 : D == 96 ? 2 : 1, NG = D == 96 ? 2 : 1;
+  uint32_t w[8][W];
+  uint32_t so[8][NG];
+  __device__ __forceinline__ void load(const AttnArgs& a, long long base, const Tile& t, int col, int grp) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int key = t.key0 + 4 * grp + (j < 4 ? j : 12 + j);
+      const long long at = base + (long long)(key < t.end ? key : t.end - 1) * a.ldkv;
+      const uint8_t* row = static_cast<const uint8_t*>(a.v) + at / 2;
+      const uint32_t* gr = reinterpret_cast<const uint32_t*>(a.vg + at / kGroup);
+      if constexpr (D == 256) {
+        const uint2 y = *reinterpret_cast<const uint2*>(row + 8 * col);
+        w[j][0] = y.x;
+        w[j][1] = y.y;
+      } else if constexpr (D == 128) {
+        w[j][0] = *reinterpret_cast<const uint32_t*>(row + 4 * col);
+      } else {
+        w[j][0] = *reinterpret_cast<const uint16_t*>(row + 2 * col);
+        if constexpr (D == 96) w[j][1] = row[32 + col];
+      }
+      so[j][0] = gr[vdim<D, true>(0, col) / kGroup];
+      if constexpr (NG == 2) so[j][1] = gr[2];
+    }
+  }
+  __device__ __forceinline__ void again() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w[j][i]));
+  }
+  // four dimensions u, u + 1.. of the key pairs (2 i, 2 i + 1), taken from the pairs' 16-bit pieces
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int u = 0; u < (DT + 3) / 4; ++u) {
+      uint32_t r[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int word = D == 96 ? u : u / 2, gi = NG == 2 ? u : 0;
+        const uint32_t x = D >= 128 && u & 1 ? pair_hi(w[2 * i][word], w[2 * i + 1][word]) : pair_lo(w[2 * i][word], w[2 * i + 1][word]);
+        dequant4(x, __builtin_bit_cast(half2_t, pair_lo(so[2 * i][gi], so[2 * i + 1][gi])),
+                 __builtin_bit_cast(half2_t, pair_hi(so[2 * i][gi], so[2 * i + 1][gi])), r[i]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (4 * u + e < DT) f(4 * u + e, __builtin_bit_cast(half8_t, make_uint4(r[0][e], r[1][e], r[2][e], r[3][e])));
+    }
+  }
+};
+
+template <int D, bool I4, bool F32>
+__global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) {
+  constexpr int DT = D / 16, QT = D / 32, OS = D + 4;
+  // the queries' operands, and after the last tile the waves' outputs
+  __shared__ __attribute__((aligned(16))) float smem[kWaves * 16 * OS];
+  static_assert(sizeof(smem) >= (F32 ? 2 : 1) * QT * 64 * sizeof(half8_t), "the queries fit");
+  half8_t(*q_s)[QT][64] = reinterpret_cast<half8_t(*)[QT][64]>(smem);
+  float(*o_s)[16][OS] = reinterpret_cast<float(*)[16][OS]>(smem);
+  __shared__ float m_s[kWaves][16], l_s[kWaves][16];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int col = lane & 15, grp = lane >> 4;
+  const int z = blockIdx.x % a.splits, bg = blockIdx.x / a.splits;
+  const int b = bg / a.KH, g = bg - b * a.KH;
+  const int m0 = blockIdx.y * 16, R = a.L * (a.H / a.KH);
+  const int p = column_pos(a, b, m0 + col);
+  const int pmax = __builtin_amdgcn_readfirstlane(row16_max(p));
+  if (pmax < 0) return;
+  const int pmin = __builtin_amdgcn_readfirstlane(-row16_max(p < 0 ? -pmax : -p));
+  const Keys keys = keys_of<kTile>(a, pmin, pmax);
+  const int per = (keys.tiles + a.splits - 1) / a.splits;
+  const int t_end = min(keys.tiles, (z + 1) * per);
+  const long long base = (long long)b * a.kvBatch + (long long)g * D;
+
+  int t = z * per + wave;
+  Tile tile = tile_of<kTile>(a, keys, t < t_end ? t : keys.tiles - 1);
+  KTile<D, I4> kx;
+  VTile<D, I4> vx;
+  if (t < t_end) {
+    kx.load(a, base, tile, col, grp);
+    vx.load(a, base, tile, col, grp);
+  }
+  Query<F32> query;
+  query.template open<D, I4>(a, b, g, m0 + col, p >= 0, grp);
+#pragma unroll
+  for (int i = 0; i < QT; ++i)
+    if (i % kWaves == wave) {
+      half8_t hi, lo;
+      query.template operand<D, I4, I4>(i, grp, hi, lo);
+      q_s[0][i][lane] = hi;
+      if constexpr (F32) q_s[1][i][lane] = lo;
+    }
+  __syncthreads();
+
+  float4_t o[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) o[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  while (t < t_end) {
+    const int tn = t + kWaves;
+    float s[8];
+    {
+      float4_t sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int i = 0; i < QT; ++i) {
+        const half8_t qh = q_s[0][i][lane];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const half8_t k8 = kx.operand(h, i, 0);
+          sc[h] = mfma(k8, qh, sc[h]);
+          if constexpr (F32) sc[h] = mfma(k8, q_s[1][i][lane], sc[h]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = sc[i >> 2][i & 3] * query.mult;
+    }
+    const Tile next = tile_of<kTile>(a, keys, tn < t_end ? tn : t);
+    if (tn < t_end) kx.load(a, base, next, col, grp);
+    if (!tile.whole) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!sees(a, p, tile.key0 + 4 * grp + (i < 4 ? i : 12 + i), tile.end)) s[i] = -INFINITY;
+    }
+    float corr;
+    const bool moves = soften(s, m, l, corr);
+    if (__builtin_amdgcn_ballot_w64(moves)) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i) o[i] *= corr;
+    }
+    half8_t ph, pl;
+    weights<F32>(s, ph, pl);
+    bool apart = false;
+    if (!tile.whole) {
+      half2_t zz = {0.f, 0.f};
+      vx.each([&](int, half8_t v) { spot(v, zz); });
+      apart = __builtin_amdgcn_ballot_w64(!(zz[0] == 0.f && zz[1] == 0.f)) != 0;
+      vx.again();
+    }
+    if (!apart) {
+      vx.each([&](int i, half8_t v) {
+        o[i] = mfma(v, ph, o[i]);
+        if constexpr (F32) o[i] = mfma(v, pl, o[i]);
+      });
+    } else {
+half8_t vis;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vis[j] = sees(a, p, tile.key0 + 4 * grp + (j < 4 ? j : 12 + j), tile.end) ? (half_t)1.f : (half_t)0.f;
+      vx.each([&](int i, half8_t v) {
+        half8_t mark;
+        v = without_marked(v, mark);
+        o[i] = mfma(v, ph, o[i]);
+        if constexpr (F32) o[i] = mfma(v, pl, o[i]);
+        o[i] = with_seen(o[i], mfma(mark, vis, float4_t{0.f, 0.f, 0.f, 0.f}));
+      });
+    }
+    if (tn < t_end) vx.load(a, base, next, col, grp);
+    tile = next;
+    t = tn;
+  }
+
+  // merge the waves: outputs by column, then whole rows
+  l = column_sum(l);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o_s[wave][col][vdim<D, I4>(i, 4 * grp + r)] = o[i][r];
+  if (grp == 0) {
+    m_s[wave][col] = m;
+    l_s[wave][col] = l;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x * 4; e < 16 * D; e += 256 * 4) {
+    const int c = e / D, d = e - c * D;
+    const int mc = m0 + c;
+    if (mc >= R) break;
+    float top = m_s[0][c];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_s[w][c]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, r[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(m_s[w][c] - ref);
+      sum += f * l_s[w][c];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] += f * o_s[w][c][d + i];
+    }
+    const int G = a.H / a.KH, i = mc / G;
+    if (a.splits > 1) {
+      const long long row = ((long long)z * a.batch * a.KH + bg) * R + mc;
+      *reinterpret_cast<float4*>(a.part_o + row * D + d) = make_float4(r[0], r[1], r[2], r[3]);
+      if (d == 0) a.part_s[row] = make_float2(top, sum);
+    } else {
+      if (column_pos(a, b, mc) < 0) continue;
+      const float inv = 1.f / sum;
+      const long long at = ((long long)b * a.L + i) * a.ldo + (long long)(g * G + mc - i * G) * D + d;
+      if constexpr (F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = make_float4(r[0] * inv, r[1] * inv, r[2] * inv, r[3] * inv);
+      } else {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack_half2(r[0] * inv, r[1] * inv), pack_half2(r[2] * inv, r[3] * inv));
+      }
+    }
+  }
+}
+
+}  // namespace
+
+int ns2cache::launch_rows(const AttnArgs& a, int D, hipStream_t s) {
+  const dim3 grid((unsigned)(a.batch * a.KH * a.splits), (unsigned)((a.L * (a.H / a.KH) + 15) / 16));
+#define NS2_ROWS(D_)                                                                             \
+  if (a.kg && !a.q_fmt) cache_rows_kernel<D_, true, true><<<grid, 64 * kWaves, 0, s>>>(a);        \
+  else if (a.kg) cache_rows_kernel<D_, true, false><<<grid, 64 * kWaves, 0, s>>>(a);              \
+  else if (!a.q_fmt) cache_rows_kernel<D_, false, true><<<grid, 64 * kWaves, 0, s>>>(a);          \
+  else cache_rows_kernel<D_, false, false><<<grid, 64 * kWaves, 0, s>>>(a);
+  NS2_CACHE_D(D, NS2_ROWS)
+#undef NS2_ROWS
+  NS2_LAUNCHED("cache_rows");
+  return NS2_OK;
+}
