@@ -2,6 +2,8 @@
 //
 // W[n][k] = scale[n][k / G] * (code[n][k] - 8), codes 0..15 two to a byte (the even column in the
 // low four bits), one fp16 scale per G = 32, 64 or 128 columns of a row.
+#include <algorithm>
+
 #include "ns2_common.h"
 
 using namespace ns2dev;
@@ -20,7 +22,14 @@ struct I4Args {
   int lda, ldc, M, N, K, group;
   float alpha;
   int act, resid;
+  int slab;  // columns of k whose rows of x are in LDS at a time
 };
+
+// The power of two that takes a row's largest magnitude to below 2^14.
+__device__ __forceinline__ int i4_up(float top) {
+  const int up = 14 - __builtin_amdgcn_frexp_expf(top);
+  return top > 0.f && top < INFINITY ? (up < 120 ? up : 120) : 0;
+}
 
 // Epilogue of one output element, as every linear's (gemm.js:159-164).
 __device__ __forceinline__ void store_i4(const I4Args& p, int m, int n, float acc, float bi, float gt) {
@@ -33,43 +42,278 @@ __device__ __forceinline__ void store_i4(const I4Args& p, int m, int n, float ac
   else *c = *c + gt * r;
 }
 
-// One wave per output column, 32 columns of k (16 bytes of codes, inside one group) per lane and
-// step, four rows of A per pass over the weights.
-template <bool A16>
-__global__ __launch_bounds__(256) void linear_i4_kernel(I4Args p) {
-  const int lane = threadIdx.x & 63;
-  const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (n >= p.N) return;
-  const uint8_t* wr = p.W + (long long)n * (p.K / 2);
-  const half_t* sr = p.scale + (long long)n * (p.K / p.group);
-  const float bi = p.bias ? p.bias[n] : 0.f;
-  const float gt = p.gate ? p.gate[p.gOff + n] : 1.f;
-  for (int m0 = 0; m0 < p.M; m0 += 4) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = lane * 32; k < p.K; k += 2048) {
-      const uint4 w4 = *reinterpret_cast<const uint4*>(wr + k / 2);
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      const float s = (float)sr[k / p.group];
+// ---- the product --------------------------------------------------------------------------------
+//
+// v_mfma_f32_16x16x32_f16 with A = 16 rows of x, B = 16 columns of W^T as the exact halves code - 8, so that a
+// product over one group needs its scale only once, in fp32, after the sum. An fp32 row of x is scaled by a
+// power of two to below 2^14 and split into two halves that keep 22 of its bits (two products); fp16 rows go in
+// as they are. The weights bound it where rows are few: 16 weight rows are read 64 bytes of each at a time (16
+// per lane, 128 columns of k, a "chunk"), and since the four lanes of a row then hold one 32-column step each
+// where the product wants a quarter of each step, the words change lanes (4 x 4, four row swaps). Within a
+// word, codes come out in the order 0 4 1 5 2 6 3 7; x is stored in that order.
+//
+// A row of A and the same row of D are apart: row 4 a + b of A is x row a + 4 b, whose results are then register
+// b of lane group a, so that up to 4 (8) rows take only one (two) of the four result registers through the
+// scales.
+
+// Four registers of the four 16-lane rows transposed: register j of row g becomes register g of row j.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) { asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) { asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
+#pragma clang diagnostic pop
+__device__ __forceinline__ void transpose_rows(uint32_t w[4]) {
+  swap32(w[0], w[2]);
+  swap32(w[1], w[3]);
+  swap16(w[0], w[1]);
+  swap16(w[2], w[3]);
+}
+
+// code - 8 of a word's eight codes: 0x6400 | c is the half 1024 + c.
+__device__ __forceinline__ half8_t codes8(uint32_t w) {
+  uint32_t r[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int m = m0 + i < p.M ? m0 + i : p.M - 1;
-        float t = 0.f;
+  for (int i = 0; i < 4; ++i)
+    r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - half2_t{1032.f, 1032.f});
+  return __builtin_bit_cast(half8_t, make_uint4(r[0], r[1], r[2], r[3]));
+}
+
+constexpr int kWaves = 4;
+constexpr int kChunk = 128;            // columns of k per load
+constexpr int kSlabBytes = 48 * 1024;  // LDS for the rows of x
+
+// A block takes 16 RT rows and, with WK = 1, 64 CT columns (16 CT per wave) over all of K; with WK = 4, 16 CT
+// columns whose chunks its waves take in turn and add up at the end. NR: result registers in use (4 NR rows of
+// each 16). SG: 32-column steps per group. The block's rows of x go to LDS a slab of p.slab columns at a time:
+// operand (step, lane group, row), `rows` rows, hi then lo.
+template <bool A16, int SG, int RT, int NR, int CT, int WK>
+__global__ __launch_bounds__(64 * kWaves) void linear_i4_kernel(I4Args p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  half8_t* x_s = reinterpret_cast<half8_t*>(smem);
+  __shared__ uint32_t top_s[16 * RT];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int c16 = lane & 15, g = lane >> 4;
+  const int m0 = blockIdx.y * (16 * RT);
+  const int rows = p.M - m0 < 16 * RT ? p.M - m0 : 16 * RT;
+  const int n0 = (WK == 1 ? blockIdx.x * kWaves + wave : blockIdx.x) * (16 * CT);
+  const int kb = p.K / 2, kg = p.K / (32 * SG);
+
+  const uint8_t* wr[CT];
+  const half_t* sr[CT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+  for (int c = 0; c < CT; ++c) {
+    const int n = n0 + 16 * c + c16 < p.N ? n0 + 16 * c + c16 : p.N - 1;
+    wr[c] = p.W + (long long)n * kb;
+    sr[c] = p.scale + (long long)n * kg;
+  }
+  uint4 w[CT];
+  half_t sc[CT];
+  auto load = [&](int chunk) {
+    int k = chunk * kChunk + 32 * g;
+    k = k < p.K ? k : 0;  // (a step past K is not used)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const long long at = (long long)m * p.lda + k + 8 * j + e;
-            const float x = A16 ? (float)static_cast<const half_t*>(p.A)[at] : static_cast<const float*>(p.A)[at];
-            t = fmaf(x, (float)((int)((w[j] >> (4 * e)) & 15) - 8), t);
+    for (int c = 0; c < CT; ++c) {
+      w[c] = *reinterpret_cast<const uint4*>(wr[c] + k / 2);
+      sc[c] = sr[c][k / (32 * SG)];
+    }
+  };
+  const int chunks = (p.K + kChunk - 1) / kChunk;
+  int chunk = WK == 1 ? 0 : wave;
+  if (chunk < chunks) load(chunk);
+
+  float tot[RT][CT][NR];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int r = 0; r < NR; ++r) tot[i][c][r] = 0.f;
+
+  // this lane's rows: of the A operand, and of the results
+  int arow[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int r = 16 * i + (c16 >> 2) + 4 * (c16 & 3);
+    arow[i] = r < rows ? r : rows - 1;
+  }
+
+  for (int k0 = 0; k0 < p.K; k0 += p.slab) {
+    const int ks = p.K - k0 < p.slab ? p.K - k0 : p.slab;
+    const int n8 = ks / 8, items = rows * n8;
+    half8_t* lo_s = x_s + items;
+    if (k0) __syncthreads();  // the last slab is used
+    if constexpr (A16) {
+      for (int u = threadIdx.x; u < items; u += 64 * kWaves) {
+        const int r = u / n8, k8 = u - r * n8;
+        const half8_t x = *reinterpret_cast<const half8_t*>(static_cast<const half_t*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8);
+        x_s[k8 * rows + r] = half8_t{x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
+      }
+    } else {
+      for (int u = threadIdx.x; u < rows; u += 64 * kWaves) top_s[u] = 0u;
+      __syncthreads();
+      for (int u = threadIdx.x; u < items; u += 64 * kWaves) {
+        const int r = u / n8, k8 = u - r * n8;
+        const float* a = static_cast<const float*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8;
+        const float4 y = *reinterpret_cast<const float4*>(a), z = *reinterpret_cast<const float4*>(a + 4);
+        const float top = fmaxf(fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))),
+                                fmaxf(fmaxf(fabsf(z.x), fabsf(z.y)), fmaxf(fabsf(z.z), fabsf(z.w))));
+        atomicMax(&top_s[r], __builtin_bit_cast(uint32_t, top));  // magnitudes order as their bits do
+      }
+      __syncthreads();
+      for (int u = threadIdx.x; u < items; u += 64 * kWaves) {
+        const int r = u / n8, k8 = u - r * n8;
+        const float* a = static_cast<const float*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8;
+        const float4 y = *reinterpret_cast<const float4*>(a), z = *reinterpret_cast<const float4*>(a + 4);
+        const float v[8] = {y.x, z.x, y.y, z.y, y.z, z.z, y.w, z.w};
+        const int up = i4_up(__builtin_bit_cast(float, top_s[r]));
+        half8_t hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float t = ldexpf(v[e], up);
+          hi[e] = (half_t)t;
+          lo[e] = (half_t)(t - (float)hi[e]);
+        }
+        x_s[k8 * rows + r] = hi;
+        lo_s[k8 * rows + r] = lo;
+      }
+    }
+    __syncthreads();
+
+    float acc[RT][CT][NR];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) acc[i][c][r] = 0.f;
+    const int last = (k0 + ks + kChunk - 1) / kChunk;
+    for (; chunk < last; chunk += WK) {
+      uint32_t t[CT][4];
+      float s[CT][4];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        t[c][0] = w[c].x;
+        t[c][1] = w[c].y;
+        t[c][2] = w[c].z;
+        t[c][3] = w[c].w;
+        const float f = (float)sc[c];
+        uint32_t a = __builtin_bit_cast(uint32_t, f), b = a;
+        swap32(a, b);  // the scales of steps 0, 1 | 2, 3
+        uint32_t a1 = a, b1 = b;
+        swap16(a, a1);
+        swap16(b, b1);
+        s[c][0] = __builtin_bit_cast(float, a);
+        s[c][1] = __builtin_bit_cast(float, a1);
+        s[c][2] = __builtin_bit_cast(float, b);
+        s[c][3] = __builtin_bit_cast(float, b1);
+      }
+      if (chunk + WK < chunks) load(chunk + WK);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) transpose_rows(t[c]);
+      const int base = (chunk * kChunk - k0) / 8 + g;
+      float4_t d[RT][CT];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (chunk * kChunk + 32 * j < k0 + ks) {  // uniform
+          half8_t xh[RT], xl[RT];
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            xh[i] = x_s[(base + 4 * j) * rows + arow[i]];
+            if constexpr (!A16) xl[i] = lo_s[(base + 4 * j) * rows + arow[i]];
           }
-        acc[i] = fmaf(t, s, acc[i]);
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            const half8_t q = codes8(t[c][j]);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+              if (j % SG == 0) d[i][c] = float4_t{0.f, 0.f, 0.f, 0.f};
+              d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[i], q, d[i][c], 0, 0, 0);
+              if constexpr (!A16) d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[i], q, d[i][c], 0, 0, 0);
+              if (j % SG == SG - 1) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) acc[i][c][r] = fmaf(s[c][j], d[i][c][r], acc[i][c][r]);
+              }
+            }
+          }
+        }
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float sum = wave_sum(acc[i]);
-      if (lane == 0 && m0 + i < p.M) store_i4(p, m0 + i, n, sum, bi, gt);
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        float back = 1.f;
+        if constexpr (!A16) {
+          const int row = 16 * i + g + 4 * r;
+          back = ldexpf(1.f, -i4_up(__builtin_bit_cast(float, top_s[row < rows ? row : rows - 1])));
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) tot[i][c][r] = fmaf(acc[i][c][r], back, tot[i][c][r]);
+      }
+  }
+
+  if constexpr (WK > 1) {
+    float* red = reinterpret_cast<float*>(smem);  // [wave][i][c][r][lane]
+    constexpr int T = RT * CT * NR;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) red[(wave * T + (i * CT + c) * NR + r) * 64 + lane] = tot[i][c][r];
+    __syncthreads();
+    for (int u = wave; u < T; u += kWaves) {
+      float sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) sum += red[(v * T + u) * 64 + lane];
+      const int r = u % NR, c = u / NR % CT, i = u / NR / CT;
+      const int m = m0 + 16 * i + g + 4 * r, n = n0 + 16 * c + c16;
+      if (m < m0 + rows && n < p.N) store_i4(p, m, n, sum, p.bias ? p.bias[n] : 0.f, p.gate ? p.gate[p.gOff + n] : 1.f);
     }
+  } else {
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const int n = n0 + 16 * c + c16;
+      if (n < p.N) {
+        const float bi = p.bias ? p.bias[n] : 0.f, gt = p.gate ? p.gate[p.gOff + n] : 1.f;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            const int m = m0 + 16 * i + g + 4 * r;
+            if (m < m0 + rows) store_i4(p, m, n, tot[i][c][r], bi, gt);
+          }
+      }
+    }
+  }
+}
+
+template <bool A16, int SG, int RT, int NR, int CT, int WK>
+void launch_i4(I4Args p, hipStream_t s) {
+  const int rows = p.M < 16 * RT ? p.M : 16 * RT, per = rows * (A16 ? 2 : 4);  // bytes of a column of k
+  p.slab = kSlabBytes / per / kChunk * kChunk;
+  if (p.slab > p.K) p.slab = p.K;
+  const size_t red = WK > 1 ? sizeof(float) * kWaves * RT * CT * NR * 64 : 0;
+  const size_t lds = std::max<size_t>((size_t)p.slab * per, red);
+  const int cols = 16 * CT * (WK == 1 ? kWaves : 1);
+  const dim3 grid((unsigned)((p.N + cols - 1LL) / cols), (unsigned)((p.M + 16 * RT - 1) / (16 * RT)));
+  linear_i4_kernel<A16, SG, RT, NR, CT, WK><<<grid, 64 * kWaves, lds, s>>>(p);
+}
+
+template <bool A16, int SG>
+void choose_i4(const I4Args& p, hipStream_t s) {
+  const long long tiles = (p.N + 15) / 16;
+  if (p.M <= 16) {
+    // one wave per 64 columns where that fills the chip, else the chunks of 16 columns over four waves
+    const bool wide = tiles >= 4 * 1024;
+    if (p.M <= 4) wide ? launch_i4<A16, SG, 1, 1, 4, 1>(p, s) : launch_i4<A16, SG, 1, 1, 1, 4>(p, s);
+    else if (p.M <= 8) wide ? launch_i4<A16, SG, 1, 2, 4, 1>(p, s) : launch_i4<A16, SG, 1, 2, 1, 4>(p, s);
+    else wide ? launch_i4<A16, SG, 1, 4, 4, 1>(p, s) : launch_i4<A16, SG, 1, 4, 1, 4>(p, s);
+  } else if (tiles * ((p.M + 31) / 32) < 2048) {
+    launch_i4<A16, SG, 2, 4, 1, 4>(p, s);
+  } else {
+    launch_i4<A16, SG, 4, 4, 2, 1>(p, s);
   }
 }
 
@@ -140,12 +384,14 @@ int ns2_linear_i4(const void* A, int a_fmt, int lda, const uint8_t* W, const uin
   NS2_REQUIRE(act >= NS2_ACT_NONE && act <= NS2_ACT_GELU_TANH, "%s: unknown activation %d", fn, act);
   NS2_REQUIRE(aligned(A, 16) && lda % (a_fmt ? 8 : 4) == 0 && aligned(W, 16) && aligned(scale, 2),
               "%s: the rows of A and W must be 16-byte aligned (lda a multiple of %d)", fn, a_fmt ? 8 : 4);
+  NS2_REQUIRE(M <= 16LL * 65535, "%s: M=%d is too many rows for one launch", fn, M);
   I4Args p{A,  W,   reinterpret_cast<const half_t*>(scale), bias, add, C, gate, cOff, gOff, lda, ldc, M, N, K, group, alpha,
            act, resid};
   ns2::ProfScope prof_("linear_i4");
-  const unsigned grid = (unsigned)((N + 3LL) / 4);
-  if (a_fmt) linear_i4_kernel<true><<<grid, 256, 0, ns2::stream()>>>(p);
-  else linear_i4_kernel<false><<<grid, 256, 0, ns2::stream()>>>(p);
+  hipStream_t s = ns2::stream();
+  if (group == 32) a_fmt ? choose_i4<true, 1>(p, s) : choose_i4<false, 1>(p, s);
+  else if (group == 64) a_fmt ? choose_i4<true, 2>(p, s) : choose_i4<false, 2>(p, s);
+  else a_fmt ? choose_i4<true, 4>(p, s) : choose_i4<false, 4>(p, s);
   NS2_LAUNCHED("linear_i4");
   return NS2_OK;
 }
