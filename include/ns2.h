@@ -277,7 +277,7 @@ int ns2_attention_rows_f16kv_oproj(const float* q, const uint16_t* k, const uint
  * v_groups an fp16 step s and offset o (2 halfs) per 32 values; such a cache stands for the fp16
  * values half(o + code * s). D is 64, 96, 128 or 256. q_fmt is the type of q (and o): 0 fp32, 1 fp16.
  * Rows of X, q, o and the cache are 16-byte aligned (ldkv, kvBatch multiples of 8 for fp16, of 32
- * for 4 bits).
+ * for 4 bits); ldkv is at most 2^24.
  *
  * ns2_head_norm_cache: X fp32 [batch*L, ldx] holds H query heads, KH key heads and KH value heads
  * (a q|k|v product). Query and key heads are RMS-normed with w_q / w_k [D] (NULL: not normed) and,

@@ -136,8 +136,29 @@ __device__ __forceinline__ Tile tile_of(const AttnArgs& a, const Keys& k, int t)
   return r;
 }
 
-__device__ __forceinline__ bool sees(const AttnArgs& a, int p, int key, int end) {
-  return key < end && key <= p && (!a.window || key > p - a.window || key < a.sinks);
+// What a column at position p (-1: nothing) sees of a tile: keys [from, from + n) and keys below `below`. (In a
+// tile of first tokens, those below its end; else its window, and first tokens that lie inside another
+// column's window.)
+struct Sight {
+  int from;
+  unsigned n;
+  int below;
+  __device__ __forceinline__ bool operator()(int key) const { return (unsigned)(key - from) < n || key < below; }
+};
+__device__ __forceinline__ Sight sight_of(const AttnArgs& a, const Keys& k, int t, int p) {
+  const bool first = t < k.tiles_first;
+  const int from = a.window && p >= a.window ? p - a.window + 1 : 0;
+  Sight s;
+  s.from = from;
+  s.n = first ? 0u : (unsigned)(p + 1 - from);
+  s.below = min(first ? k.first : a.sinks, p + 1);
+  return s;
+}
+
+// A tile's first row, from which lanes count in 32 bits (rows are at most 2^24 values apart).
+__device__ __forceinline__ const char* tile_rows(const void* cache, long long base, int key0, int ldkv, bool i4) {
+  const long long at = base + (long long)key0 * ldkv;
+  return static_cast<const char*>(cache) + (i4 ? at / 2 : at * 2);
 }
 
 // ---- queries -------------------------------------------------------------------------------------
@@ -205,8 +226,10 @@ struct Query {
 // ---- the softmax's running state -------------------------------------------------------------------
 
 // The reference m of a column trails its maximum by up to 2^kSlack: only a score above m + kSlack moves it
-// and rescales the sums, so that most tiles leave the accumulators alone. Weights are then at most 2^kSlack.
-constexpr float kSlack = 8.f;
+// and rescales the sums, so that most tiles leave the accumulators alone. Weights are 2^(score - m + kLift),
+// at most 2^(kSlack + kLift): far enough below fp16's largest value, and as far as that allows above its
+// smallest (a weight's rounding is off by 2^-25 at least, 2^-31 of the weight of the reference).
+constexpr float kSlack = 8.f, kLift = 6.f;
 
 // Scores s[N] (base-2 logarithms, -inf where masked) of the lane's column -> weights in place; returns
 // whether the lane's column moved its reference, with the factor for what was summed before.
@@ -217,12 +240,9 @@ __device__ __forceinline__ bool soften(float (&s)[N], float& m, float& l, float&
   for (int i = 1; i < N; ++i) top = fmaxf(top, s[i]);
   top = column_max(top);
   const bool moves = top > m + kSlack;
-  corr = 1.f;
-  if (moves) {
-    corr = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-    m = top;
-  }
-  const float ref = m == -INFINITY ? 0.f : m;
+  corr = moves && m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : moves ? 0.f : 1.f;
+  m = moves ? top : m;
+  const float ref = m == -INFINITY ? 0.f : m - kLift;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -237,19 +257,26 @@ __device__ __forceinline__ float4_t mfma(half8_t a, half8_t b, float4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// The B operand of the second product: eight weights, as halves hi (+ lo).
+// The B operand of the second product: eight weights, rounded to halves, or (F32) as two halves: the leading
+// 11 bits and the rest, which keeps 21 to 22 bits in all.
 template <bool F32>
 __device__ __forceinline__ void weights(const float* p, half8_t& hi, half8_t& lo) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    hi[e] = (half_t)p[e];
-    if constexpr (F32) lo[e] = (half_t)(p[e] - (float)hi[e]);
+    if constexpr (!F32) {
+      hi[e] = (half_t)p[e];
+    } else {
+      const float lead = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p[e]) & 0xffffe000u);
+      hi[e] = (half_t)lead;
+      lo[e] = (half_t)(p[e] - lead);
+    }
   }
 }
 
 // Values that are not finite must reach the columns that see them and no others, but 0 * inf is NaN: they are
 // taken out of the product, and a second product of marks (1 for inf, 64 for -inf, 4096 for NaN) with the
-// columns' visible keys (1 or 0) tells each output what it has seen (at most 32 of each per product).
+// columns' visible keys (1 or 0) tells each output what it has seen (at most 32 of each per product). What was
+// seen is kept aside, one byte per output, and put into the outputs at the end.
 __device__ __forceinline__ half8_t without_marked(half8_t v, half8_t& mark) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -260,11 +287,21 @@ __device__ __forceinline__ half8_t without_marked(half8_t v, half8_t& mark) {
   }
   return v;
 }
-__device__ __forceinline__ float4_t with_seen(float4_t o, float4_t count) {
+// bits per output: 1 inf, 2 -inf, 4 NaN
+__device__ __forceinline__ uint32_t seen_bits(float4_t count) {
+  uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int c = (int)count[i], plus = c & 63, minus = (c >> 6) & 63;
-    if (c) o[i] += c >= 4096 || (plus && minus) ? NAN : plus ? INFINITY : -INFINITY;
+    const int c = (int)count[i];
+    w |= (uint32_t)((c & 63 ? 1 : 0) | (c & 0xfc0 ? 2 : 0) | (c >= 4096 ? 4 : 0)) << (8 * i);
+  }
+  return w;
+}
+__device__ __forceinline__ float4_t with_seen(float4_t o, uint32_t bits) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = (bits >> (8 * i)) & 7u;
+    if (b) o[i] += b == 1 ? INFINITY : b == 2 ? -INFINITY : NAN;
   }
   return o;
 }

@@ -129,41 +129,69 @@ __global__ __launch_bounds__(256) void cache_write_kernel(WriteArgs a) {
 
 // ---- attention: the splits joined, and which kernel runs ---------------------------------------------
 
-// One wave per column: the splits' sums weighted to their common maximum, in split order. A split that saw no
-// key has maximum -inf and its sums are not read.
-__global__ __launch_bounds__(256) void cache_join_kernel(AttnArgs a, int D) {
-  const int lane = threadIdx.x & 63;
+// One block per column: the splits' sums weighted to their common maximum. D / 4 lanes hold a row of D, so that
+// the block's Z groups of lanes take a split each, up to four at a time in flight; the groups are added in order.
+// A split that saw no key has maximum -inf and its sums are not taken.
+constexpr int kMaxSplits = 64;
+
+template <int D>
+__global__ __launch_bounds__(256) void cache_join_kernel(AttnArgs a) {
+  constexpr int T = D / 4, PW = 64 / T, Z = 4 * PW;
+  __shared__ float4 o_s[Z][T];
+  __shared__ float f_s[kMaxSplits];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int G = a.H / a.KH, R = a.L * G;
-  const long long columns = (long long)a.batch * a.KH * R, u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (u >= columns) return;
+  const long long columns = (long long)a.batch * a.KH * R, u = blockIdx.x;
   const int bg = (int)(u / R), mc = (int)(u - (long long)bg * R), b = bg / a.KH, g = bg - b * a.KH;
   if (column_pos(a, b, mc) < 0) return;
-  float top = -INFINITY;
-  for (int z = 0; z < a.splits; ++z) top = fmaxf(top, a.part_s[z * columns + u].x);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, r[4] = {0.f, 0.f, 0.f, 0.f};
-  const int d = 4 * lane;
-  for (int z = 0; z < a.splits; ++z) {
-    const float2 ml = a.part_s[z * columns + u];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-    sum += f * ml.y;
-    if (d < D) {
-      const float4 x = *reinterpret_cast<const float4*>(a.part_o + (z * columns + u) * D + d);
-      r[0] += f * x.x;
-      r[1] += f * x.y;
-      r[2] += f * x.z;
-      r[3] += f * x.w;
+  const float2 ml = lane < a.splits ? a.part_s[lane * columns + u] : make_float2(-INFINITY, 0.f);
+  float top = ml.x;
+  for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
+  const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
+  const float sum = wave_sum(f * ml.y);
+  if (wave == 0) f_s[lane] = ml.x == -INFINITY && ml.y == 0.f ? -1.f : f;
+  __syncthreads();
+  const int sub = lane / T, t = lane - sub * T, zg = wave * PW + sub;
+  float r[4] = {0.f, 0.f, 0.f, 0.f};
+  if (sub < PW) {
+    for (int z0 = zg; z0 < a.splits; z0 += 4 * Z) {
+      float4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int z = z0 + i * Z;
+        if (z < a.splits && f_s[z] >= 0.f) x[i] = *reinterpret_cast<const float4*>(a.part_o + (z * columns + u) * D + 4 * t);
+        else x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int z = z0 + i * Z;
+        const float w = z < a.splits && f_s[z] >= 0.f ? f_s[z] : 0.f;
+        r[0] += w * x[i].x;
+        r[1] += w * x[i].y;
+        r[2] += w * x[i].z;
+        r[3] += w * x[i].w;
+      }
     }
+    o_s[zg][t] = make_float4(r[0], r[1], r[2], r[3]);
   }
-  if (d >= D) return;
+  __syncthreads();
+  if (threadIdx.x >= T) return;
+  float4 q = o_s[0][t];
+#pragma unroll
+  for (int i = 1; i < Z; ++i) {
+    const float4 x = o_s[i][t];
+    q.x += x.x;
+    q.y += x.y;
+    q.z += x.z;
+    q.w += x.w;
+  }
   const float inv = 1.f / sum;
   const int i = mc / G;
-  const long long at = ((long long)b * a.L + i) * a.ldo + (long long)(g * G + mc - i * G) * D + d;
+  const long long at = ((long long)b * a.L + i) * a.ldo + (long long)(g * G + mc - i * G) * D + 4 * t;
   if (a.q_fmt)
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack_half2(r[0] * inv, r[1] * inv), pack_half2(r[2] * inv, r[3] * inv));
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = make_uint2(pack_half2(q.x * inv, q.y * inv), pack_half2(q.z * inv, q.w * inv));
   else
-    *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = make_float4(r[0] * inv, r[1] * inv, r[2] * inv, r[3] * inv);
+    *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = make_float4(q.x * inv, q.y * inv, q.z * inv, q.w * inv);
 }
 
 constexpr int kRowsColumns = 64;  // columns of a K/V head up to which its keys are streamed past 16 at a time
@@ -178,7 +206,7 @@ Plan plan_of(int batch, int L, int H, int KH, int cap, int window, int sinks) {
   const long long blocks = heads * (p.prompt ? (R + 63) / 64 : (R + 15) / 16);
   const long long want = p.prompt ? kCUs / blocks : 2 * kCUs / blocks;
   // at least four tiles of 64 keys, or two of 32 for each of four waves, per split
-  const long long most = std::max<long long>(1, keys / 256);
+  const long long most = std::min<long long>(kMaxSplits, std::max<long long>(1, keys / 256));
   p.splits = (int)std::max<long long>(1, std::min(want, most));
   return p;
 }
@@ -190,7 +218,8 @@ int check_cache(const char* fn, const void* q, const int* pos, const void* k, co
   NS2_REQUIRE(D == 64 || D == 96 || D == 128 || D == 256, "%s: head dim %d is not 64, 96, 128 or 256", fn, D);
   NS2_REQUIRE(H > 0 && KH > 0 && H % KH == 0 && (long long)H * D <= INT32_MAX, "%s: H=%d is not a positive multiple of KH=%d", fn, H,
               KH);
-  NS2_REQUIRE(cap > 0 && ldq >= H * D && ldkv >= (long long)KH * D && kvBatch >= 0, "%s: bad sizes or strides", fn);
+  NS2_REQUIRE(cap > 0 && ldq >= H * D && ldkv >= (long long)KH * D && ldkv <= 1 << 24 && kvBatch >= 0,
+              "%s: bad sizes or strides (cap=%d, ldq=%d, ldkv=%d)", fn, cap, ldq, ldkv);
   NS2_REQUIRE(!kg == !vg, "%s: a 4-bit cache needs the groups of both k and v", fn);
   NS2_REQUIRE(q_fmt == 0 || q_fmt == 1, "%s: q_fmt %d is not 0 (fp32) or 1 (fp16)", fn, q_fmt);
   NS2_REQUIRE(aligned(q, 16) && ldq % (q_fmt ? 8 : 4) == 0 && aligned(pos, 4), "%s: the rows of q must be 16-byte aligned", fn);
@@ -288,7 +317,9 @@ int ns2_attention_cache(const void* q, int q_fmt, int ldq, const int* pos, const
   if (int rc = plan.prompt ? launch_prompt(a, D, s) : launch_rows(a, D, s)) return rc;
   if (plan.splits > 1) {
     const long long columns = (long long)batch * L * H;
-    cache_join_kernel<<<(unsigned)((columns + 3) / 4), 256, 0, s>>>(a, D);
+#define NS2_JOIN(D_) cache_join_kernel<D_><<<(unsigned)columns, 256, 0, s>>>(a);
+    NS2_CACHE_D(D, NS2_JOIN)
+#undef NS2_JOIN
     NS2_LAUNCHED("cache_join");
   }
   return NS2_OK;

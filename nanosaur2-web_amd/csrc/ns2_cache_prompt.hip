@@ -1,12 +1,14 @@
 // Attention of many query columns over a cache: prompts and their continuations.
 //
-// The two products bound it. A block takes 64 CT columns of one K/V head (CT tiles of 16 in each of its four
-// waves, queries and accumulators in registers) and runs over the keys they see in tiles of 64. A tile's K
-// and V rows go to LDS once for all waves, as operand fragments: K as it lies, V transposed in registers on
-// the way (8 keys x 8 dimensions per thread, one byte permutation per pair of values), 4-bit values turned
-// into fp16 there. The next tile's rows are requested before this one's products. Fragments are 1 KB, lane by
-// lane; the 16-byte slots inside one are exchanged (xor) by a pattern of the fragment so that the threads
-// of a row write to different banks.
+// The two products bound it. A block takes 64 CT columns of one K/V head and runs over the keys they see in
+// tiles of 64. Its eight waves are four groups of columns (CT tiles of 16 each, queries and accumulators in
+// registers) times two halves of every tile, with a softmax state each; the halves are merged at the end. So
+// every SIMD has two waves to choose from where one block fills a CU, and a wave reads from LDS only its half
+// of a tile. A tile's K and V rows go to LDS once for all waves, as operand fragments, while four waves bring
+// K and four V: K as it lies, V transposed in registers on the way (8 keys x VD dimensions per thread, one byte
+// permutation per pair of values), 4-bit values turned into fp16 there. The next tile's rows are requested
+// before this one's products. Fragments are 1 KB, lane by lane; the 16-byte slots inside one are exchanged
+// (xor) by a pattern of the fragment so that the threads of a row write to different banks.
 #include "ns2_cache.h"
 
 using namespace ns2cache;
@@ -14,119 +16,131 @@ using namespace ns2cache;
 namespace {
 
 constexpr int kTile = 64;  // keys
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
+constexpr int kHalf = 256;  // threads that bring K, and V
 
-// What one thread brings of a tile from memory to LDS: NK pieces of 8 dimensions of a K row and NV blocks of
-// 8 keys x 8 dimensions of V.
+// What one thread brings of a tile from memory to LDS: NK pieces of 8 dimensions of K rows, or one block of
+// 8 keys x VD dimensions of V.
 template <int D, bool I4>
 struct Stage {
-  static constexpr int C = D / 8;                                 // 8-dimension pieces of a row
-  static constexpr int NK = (kTile * C + kThreads - 1) / kThreads;  // pieces of K per thread
-  static constexpr int VB = 8 * C;                                // 8x8 blocks of V
-  static constexpr int NV = (VB + kThreads - 1) / kThreads;
-  typename std::conditional<I4, uint32_t, uint4>::type k[NK], v[NV][8];
-  uint32_t ks[I4 ? NK : 1], vs[I4 ? NV : 1][8];
+  static constexpr int C = D / 8, NK = kTile * C / kHalf;  // 8-dimension pieces of a row; of K per thread
+  static constexpr int VD = D == 256 ? 8 : D >= 96 ? 4 : 2, VC = D / VD;
+  static constexpr int NR = I4 ? 8 : NK * 4 > 4 * VD ? NK * 4 : 4 * VD;
+  static_assert(kTile * C % kHalf == 0 && 8 * VC <= kHalf && NK <= 8, "thread shares");
+  uint32_t raw[NR], group[I4 ? 8 : 1];
 
-  __device__ __forceinline__ void load(const AttnArgs& a, long long base, const Tile& t) {
-    const int tid = threadIdx.x;
+  __device__ __forceinline__ void load_k(const AttnArgs& a, long long base, const Tile& t, int tid) {
+    const char* rows = tile_rows(a.k, base, t.key0, a.ldkv, I4);
+    const int last = t.end - 1 - t.key0;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-      const int u = tid + kThreads * i, key = t.key0 + u / C, c = u % C;
-      if (kTile * C % kThreads == 0 || u < kTile * C) {
-        const long long at = base + (long long)(key < t.end ? key : t.end - 1) * a.ldkv + 8 * c;
-        if constexpr (I4) {
-          k[i] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.k) + at / 2);
-          ks[i] = reinterpret_cast<const uint32_t*>(a.kg)[at / kGroup];
-        } else {
-          k[i] = *reinterpret_cast<const uint4*>(static_cast<const half_t*>(a.k) + at);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int u = tid + kThreads * i, c = u % C, q = u / C;  // q = 4 (key step) + lane group
-      if (VB % kThreads == 0 || u < VB) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int key = t.key0 + 32 * (q >> 2) + 4 * (q & 3) + (j < 4 ? j : 12 + j);
-          const long long at = base + (long long)(key < t.end ? key : t.end - 1) * a.ldkv + 8 * c;
-          if constexpr (I4) {
-            v[i][j] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + at / 2);
-            vs[i][j] = reinterpret_cast<const uint32_t*>(a.vg)[at / kGroup];
-          } else {
-            v[i][j] = *reinterpret_cast<const uint4*>(static_cast<const half_t*>(a.v) + at);
-          }
-        }
+      const int u = tid + kHalf * i, key = min(u / C, last), c = u % C;
+      const uint32_t at = (uint32_t)(key * a.ldkv + 8 * c);
+      if constexpr (I4) {
+        raw[i] = *reinterpret_cast<const uint32_t*>(rows + at / 2);
+        group[i] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(a.kg) + (base + (long long)t.key0 * a.ldkv) / kGroup * 4 + at / kGroup * 4);
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(rows + 2u * at);
+        raw[4 * i] = x.x;
+        raw[4 * i + 1] = x.y;
+        raw[4 * i + 2] = x.z;
+        raw[4 * i + 3] = x.w;
       }
     }
   }
 
-  // K fragment (key tile kt, step t): lane (key % 16, grp) holds dimensions 32 t + 8 grp ..; V fragment (step t,
-  // key step ks): lane (dimension % 16, grp) holds the eight keys of grp. Returns NaN if a V value is not finite.
-  __device__ __forceinline__ half2_t store(half8_t* ksm, half8_t* vsm, bool check) const {
-    const int tid = threadIdx.x;
-    half2_t z = {0.f, 0.f};
+  __device__ __forceinline__ void load_v(const AttnArgs& a, long long base, const Tile& t, int tid) {
+    if (8 * VC < kHalf && tid >= 8 * VC) return;
+    const char* rows = tile_rows(a.v, base, t.key0, a.ldkv, I4);
+    const int last = t.end - 1 - t.key0;
+    const int c = tid % VC, q = tid / VC;  // q = 4 (tile half) + lane group
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const int u = tid + kThreads * i, key = u / C, c = u % C;
-      if (kTile * C % kThreads == 0 || u < kTile * C) {
-        half8_t x;
-        if constexpr (I4) x = dequant8(k[i], __builtin_bit_cast(half2_t, ks[i]));
-        else x = __builtin_bit_cast(half8_t, k[i]);
-        ksm[((key >> 4) * (D / 32) + (c >> 2)) * 64 + (c & 3) * 16 + ((key ^ c) & 15)] = x;
+    for (int j = 0; j < 8; ++j) {
+      const int key = min(32 * (q >> 2) + 4 * (q & 3) + (j < 4 ? j : 12 + j), last);
+      const uint32_t at = (uint32_t)(key * a.ldkv + VD * c);
+      if constexpr (I4) {
+        raw[j] = VD == 8   ? *reinterpret_cast<const uint32_t*>(rows + at / 2)
+                 : VD == 4 ? *reinterpret_cast<const uint16_t*>(rows + at / 2)
+                           : *reinterpret_cast<const uint8_t*>(rows + at / 2);
+        group[j] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(a.vg) + (base + (long long)t.key0 * a.ldkv) / kGroup * 4 + at / kGroup * 4);
+      } else if constexpr (VD == 8) {
+        const uint4 x = *reinterpret_cast<const uint4*>(rows + 2u * at);
+        raw[4 * j] = x.x;
+        raw[4 * j + 1] = x.y;
+        raw[4 * j + 2] = x.z;
+        raw[4 * j + 3] = x.w;
+      } else if constexpr (VD == 4) {
+        const uint2 x = *reinterpret_cast<const uint2*>(rows + 2u * at);
+        raw[2 * j] = x.x;
+        raw[2 * j + 1] = x.y;
+      } else {
+        raw[j] = *reinterpret_cast<const uint32_t*>(rows + 2u * at);
       }
     }
+  }
+
+  // K fragment (key tile kt, step t): lane (key % 16, grp) holds dimensions 32 t + 8 grp ..
+  __device__ __forceinline__ void store_k(half8_t* ksm, int tid) const {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int u = tid + kThreads * i, c = u % C, q = u / C;
-      if (VB % kThreads == 0 || u < VB) {
-        uint32_t r[8][4];  // [dimension][key pair]
-        if constexpr (I4) {
+    for (int i = 0; i < NK; ++i) {
+      const int u = tid + kHalf * i, key = u / C, c = u % C;
+      half8_t x;
+      if constexpr (I4) x = dequant8(raw[i], __builtin_bit_cast(half2_t, group[i]));
+      else x = __builtin_bit_cast(half8_t, make_uint4(raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]));
+      ksm[((key >> 4) * (D / 32) + (c >> 2)) * 64 + (c & 3) * 16 + ((key ^ c) & 15)] = x;
+    }
+  }
+
+  // V fragment (step t, tile half): lane (dimension % 16, grp) holds the eight keys of grp. Returns NaN if a value
+  // is not finite and `check` is set.
+  __device__ __forceinline__ half2_t store_v(half8_t* vsm, int tid, bool check) const {
+    half2_t z = {0.f, 0.f};
+    if (8 * VC < kHalf && tid >= 8 * VC) return z;
+    const int c = tid % VC, q = tid / VC;
+    uint32_t r[VD][4];  // [dimension][key pair]
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const half2_t s = __builtin_bit_cast(half2_t, pair_lo(vs[i][2 * j], vs[i][2 * j + 1]));
-            const half2_t o = __builtin_bit_cast(half2_t, pair_hi(vs[i][2 * j], vs[i][2 * j + 1]));
-            uint32_t x[4], y[4];
-            dequant4(pair_lo(v[i][2 * j], v[i][2 * j + 1]), s, o, x);
-            dequant4(pair_hi(v[i][2 * j], v[i][2 * j + 1]), s, o, y);
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (I4) {
+        const half2_t s = __builtin_bit_cast(half2_t, pair_lo(group[2 * j], group[2 * j + 1]));
+        const half2_t o = __builtin_bit_cast(half2_t, pair_hi(group[2 * j], group[2 * j + 1]));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              r[e][j] = x[e];
-              r[4 + e][j] = y[e];
-            }
-          }
-        } else {
+        for (int h = 0; h < (VD + 3) / 4; ++h) {
+          uint32_t x[4];
+          dequant4(h ? pair_hi(raw[2 * j], raw[2 * j + 1]) : pair_lo(raw[2 * j], raw[2 * j + 1]), s, o, x);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t x[4] = {v[i][2 * j].x, v[i][2 * j].y, v[i][2 * j].z, v[i][2 * j].w};
-            const uint32_t y[4] = {v[i][2 * j + 1].x, v[i][2 * j + 1].y, v[i][2 * j + 1].z, v[i][2 * j + 1].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              r[2 * e][j] = pair_lo(x[e], y[e]);
-              r[2 * e + 1][j] = pair_hi(x[e], y[e]);
-            }
-          }
+          for (int e = 0; e < 4; ++e)
+            if (4 * h + e < VD) r[4 * h + e][j] = x[e];
         }
-        const int t = c >> 1;
+      } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const half8_t x = __builtin_bit_cast(half8_t, make_uint4(r[e][0], r[e][1], r[e][2], r[e][3]));
-          if (check) spot(x, z);
-          vsm[(t * 2 + (q >> 2)) * 64 + (q & 3) * 16 + (((c & 1) * 8 + e) ^ (t & 7))] = x;
+        for (int e = 0; e < VD / 2; ++e) {
+          const uint32_t x = raw[2 * j * (VD / 2) + e], y = raw[(2 * j + 1) * (VD / 2) + e];
+          r[2 * e][j] = pair_lo(x, y);
+          r[2 * e + 1][j] = pair_hi(x, y);
         }
       }
+    }
+    const int t = VD * c >> 4;
+#pragma unroll
+    for (int e = 0; e < VD; ++e) {
+      const half8_t x = __builtin_bit_cast(half8_t, make_uint4(r[e][0], r[e][1], r[e][2], r[e][3]));
+      if (check) spot(x, z);
+      vsm[(t * 2 + (q >> 2)) * 64 + (q & 3) * 16 + (((VD * c & 15) + e) ^ (t & (VD - 1)))] = x;
     }
     return z;
   }
 };
 
 template <int D, bool I4, bool F32, int CT>
-__global__ __launch_bounds__(kThreads) void cache_prompt_kernel(AttnArgs a) {
-  constexpr int DT = D / 16, QT = D / 32;
-  __shared__ __attribute__((aligned(16))) half8_t k_s[4 * QT * 64];
-  __shared__ __attribute__((aligned(16))) half8_t v_s[DT * 2 * 64];
-  __shared__ int bad_s;  // 1 + the last tile with a V value that is not finite
+__global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
+  constexpr int DT = D / 16, QT = D / 32, VD = Stage<D, I4>::VD;
+  constexpr int kFrags = 4 * QT + 2 * DT, kMerge = 4 * CT * (DT + 1);  // KB of a tile; of the second halves' sums
+  __shared__ __attribute__((aligned(16))) half8_t smem[(kFrags > kMerge ? kFrags : kMerge) * 64];
+  __shared__ uint32_t seen_s[8][CT * DT][64];  // values that were not finite
+  __shared__ int bad_s;                        // 1 + the last tile with such a V value
+  half8_t *k_s = smem, *v_s = smem + 4 * QT * 64;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int half = wave >> 2, tid = threadIdx.x & (kHalf - 1);  // waves 0-3: first half of a tile, bring K
   const int col = lane & 15, grp = lane >> 4;
   const int G = a.H / a.KH, R = a.L * G;
   const int z = blockIdx.x % a.splits, bg = blockIdx.x / a.splits;
@@ -155,62 +169,73 @@ __global__ __launch_bounds__(kThreads) void cache_prompt_kernel(AttnArgs a) {
 
   Stage<D, I4> st;
   Tile tile = tile_of<kTile>(a, keys, t0 < t1 ? t0 : 0);
-  if (t0 < t1) st.load(a, base, tile);
+  if (t0 < t1) {
+    if (half == 0) st.load_k(a, base, tile, tid);
+    else st.load_v(a, base, tile, tid);
+  }
   half8_t qh[CT][QT], ql[CT][F32 ? QT : 1];
-  Query<F32> query[CT];
-  float m[CT], l[CT];
+  float mult[CT], m[CT], l[CT];
   int p[CT];
   float4_t o[CT][DT];
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
-    const int mc = m0 + (wave * CT + c) * 16 + col;
+    const int mc = m0 + ((wave & 3) * CT + c) * 16 + col;
     p[c] = column_pos(a, b, mc);
-    query[c].template open<D, false>(a, b, g, mc, p[c] >= 0, grp);
+    Query<F32> query;
+    query.template open<D, false>(a, b, g, mc, p[c] >= 0, grp);
+    mult[c] = query.mult;
 #pragma unroll
-    for (int i = 0; i < QT; ++i) query[c].template operand<D, false, I4>(i, grp, qh[c][i], ql[c][F32 ? i : 0]);
+    for (int i = 0; i < QT; ++i) query.template operand<D, false, I4>(i, grp, qh[c][i], ql[c][F32 ? i : 0]);
     m[c] = -INFINITY;
     l[c] = 0.f;
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[c][i] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
   if (threadIdx.x == 0) bad_s = 0;
+  bool seen = false;
 
   for (int t = t0; t < t1; ++t) {
     __syncthreads();  // the last tile's fragments are used
-    {
-      const half2_t zz = st.store(k_s, v_s, !tile.whole);
+    if (half == 0) {
+      st.store_k(k_s, tid);
+    } else {
+      const half2_t zz = st.store_v(v_s, tid, !tile.whole);
       if (!(zz[0] == 0.f && zz[1] == 0.f)) bad_s = t + 1;
     }
     __syncthreads();
     const Tile next = tile_of<kTile>(a, keys, t + 1 < t1 ? t + 1 : t);
-    if (t + 1 < t1) st.load(a, base, next);
+    if (t + 1 < t1) {
+      if (half == 0) st.load_k(a, base, next, tid);
+      else st.load_v(a, base, next, tid);
+    }
 
-    float4_t s[CT][4];
+    float4_t s[CT][2];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) s[c][kt] = float4_t{0.f, 0.f, 0.f, 0.f};
+      for (int kt = 0; kt < 2; ++kt) s[c][kt] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < QT; ++i)
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        const half8_t k8 = k_s[(kt * QT + i) * 64 + grp * 16 + ((col ^ (4 * i + grp)) & 15)];
+      for (int kt = 0; kt < 2; ++kt) {
+        const half8_t k8 = k_s[((2 * half + kt) * QT + i) * 64 + grp * 16 + ((col ^ (4 * i + grp)) & 15)];
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
           s[c][kt] = mfma(k8, qh[c][i], s[c][kt]);
           if constexpr (F32) s[c][kt] = mfma(k8, ql[c][i], s[c][kt]);
         }
       }
-    half8_t ph[CT][2], pl[CT][2];
+    half8_t ph[CT], pl[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      float w[16];
+      float w[8];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = s[c][i >> 2][i & 3] * query[c].mult;
+      for (int i = 0; i < 8; ++i) w[i] = s[c][i >> 2][i & 3] * mult[c];
       if (!tile.whole) {
+        const Sight sight = sight_of(a, keys, t, p[c]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (!sees(a, p[c], tile.key0 + 16 * (i >> 2) + 4 * grp + (i & 3), tile.end)) w[i] = -INFINITY;
+        for (int i = 0; i < 8; ++i)
+          if (!sight(tile.key0 + 32 * half + 16 * (i >> 2) + 4 * grp + (i & 3))) w[i] = -INFINITY;
       }
       float corr;
       const bool moves = soften(w, m[c], l[c], corr);
@@ -218,68 +243,91 @@ __global__ __launch_bounds__(kThreads) void cache_prompt_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[c][i] *= corr;
       }
-      weights<F32>(w, ph[c][0], pl[c][0]);
-      weights<F32>(w + 8, ph[c][1], pl[c][1]);
+      weights<F32>(w, ph[c], pl[c]);
     }
-    const bool apart = !tile.whole && bad_s == t + 1;
-    if (!apart) {
+    if (!tile.whole && bad_s == t + 1) {  // (for all waves)
+      half8_t vis[CT];
 #pragma unroll
-      for (int i = 0; i < DT; ++i)
+      for (int c = 0; c < CT; ++c) {
+        const Sight sight = sight_of(a, keys, t, p[c]);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const half8_t v8 = v_s[(i * 2 + ks) * 64 + grp * 16 + (col ^ (i & 7))];
-#pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            o[c][i] = mfma(v8, ph[c][ks], o[c][i]);
-            if constexpr (F32) o[c][i] = mfma(v8, pl[c][ks], o[c][i]);
-          }
-        }
-    } else {
+        for (int j = 0; j < 8; ++j)
+          vis[c][j] = sight(tile.key0 + 32 * half + 4 * grp + (j < 4 ? j : 12 + j)) ? (half_t)1.f : (half_t)0.f;
+      }
 #pragma unroll 1
-      for (int ks = 0; ks < 2; ++ks) {
-        half8_t vis[CT];
+      for (int i = 0; i < DT; ++i) {
+        half8_t mark;
+        without_marked(v_s[(i * 2 + half) * 64 + grp * 16 + (col ^ (i & (VD - 1)))], mark);
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            vis[c][j] = sees(a, p[c], tile.key0 + 32 * ks + 4 * grp + (j < 4 ? j : 12 + j), tile.end) ? (half_t)1.f : (half_t)0.f;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) {
-          half8_t mark;
-          const half8_t v8 = without_marked(v_s[(i * 2 + ks) * 64 + grp * 16 + (col ^ (i & 7))], mark);
-#pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            o[c][i] = mfma(v8, ks ? ph[c][1] : ph[c][0], o[c][i]);
-            if constexpr (F32) o[c][i] = mfma(v8, ks ? pl[c][1] : pl[c][0], o[c][i]);
-            o[c][i] = with_seen(o[c][i], mfma(mark, vis[c], float4_t{0.f, 0.f, 0.f, 0.f}));
-          }
+        for (int c = 0; c < CT; ++c) {
+          uint32_t* w = &seen_s[wave][c * DT + i][lane];
+          *w = (seen ? *w : 0u) | seen_bits(mfma(mark, vis[c], float4_t{0.f, 0.f, 0.f, 0.f}));
         }
+      }
+      seen = true;
+      __syncthreads();  // every wave has the marks: the values go
+#pragma unroll 1
+      for (int i = threadIdx.x; i < 2 * DT * 64; i += kThreads) {
+        half8_t mark;
+        v_s[i] = without_marked(v_s[i], mark);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      const half8_t v8 = v_s[(i * 2 + half) * 64 + grp * 16 + (col ^ (i & (VD - 1)))];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        o[c][i] = mfma(v8, ph[c], o[c][i]);
+        if constexpr (F32) o[c][i] = mfma(v8, pl[c], o[c][i]);
       }
     }
     tile = next;
   }
 
+  if (seen) {
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int i = 0; i < DT; ++i) o[c][i] = with_seen(o[c][i], seen_s[wave][c * DT + i][lane]);
+  }
+
+  // the second halves' sums through LDS to the first's
+  float4_t* o_s = reinterpret_cast<float4_t*>(smem) + (wave & 3) * (CT * DT * 64);
+  float2* ml_s = reinterpret_cast<float2*>(reinterpret_cast<float4_t*>(smem) + 4 * CT * DT * 64) + (wave & 3) * (CT * 64);
+  __syncthreads();
+  if (half) {
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i) o_s[(c * DT + i) * 64 + lane] = o[c][i];
+      ml_s[c * 64 + lane] = make_float2(m[c], l[c]);
+    }
+  }
+  __syncthreads();
+  if (half) return;
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
-    const float sum = column_sum(l[c]);
+    const float2 ml = ml_s[c * 64 + lane];
+    const float top = fmaxf(m[c], ml.x), ref = top == -INFINITY ? 0.f : top;
+    const float f0 = __builtin_amdgcn_exp2f(m[c] - ref), f1 = __builtin_amdgcn_exp2f(ml.x - ref);
+    const float sum = column_sum(f0 * l[c] + f1 * ml.y);
     const int mc = m0 + (wave * CT + c) * 16 + col;
     if (p[c] < 0) continue;
-    if (a.splits > 1) {
-      const long long row = ((long long)z * a.batch * a.KH + bg) * R + mc;
+    const int i0 = mc / G;
+    const long long row = ((long long)z * a.batch * a.KH + bg) * R + mc;
+    const long long at = ((long long)b * a.L + i0) * a.ldo + (long long)(g * G + mc - i0 * G) * D + 4 * grp;
+    const float inv = a.splits > 1 ? 1.f : 1.f / sum;
+    if (a.splits > 1 && grp == 0) a.part_s[row] = make_float2(top, sum);
 #pragma unroll
-      for (int i = 0; i < DT; ++i)
-        *reinterpret_cast<float4*>(a.part_o + row * D + 16 * i + 4 * grp) = make_float4(o[c][i][0], o[c][i][1], o[c][i][2], o[c][i][3]);
-      if (grp == 0) a.part_s[row] = make_float2(m[c], sum);
-    } else {
-      const float inv = 1.f / sum;
-      const int i0 = mc / G;
-      const long long at = ((long long)b * a.L + i0) * a.ldo + (long long)(g * G + mc - i0 * G) * D + 4 * grp;
-#pragma unroll
-      for (int i = 0; i < DT; ++i) {
-        const float4_t r = o[c][i] * inv;
-        if constexpr (F32) *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at + 16 * i) = make_float4(r[0], r[1], r[2], r[3]);
-        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at + 16 * i) = make_uint2(pack_half2(r[0], r[1]), pack_half2(r[2], r[3]));
-      }
+    for (int i = 0; i < DT; ++i) {
+      const float4_t r = (o[c][i] * f0 + o_s[(c * DT + i) * 64 + lane] * f1) * inv;
+      if (a.splits > 1)
+        *reinterpret_cast<float4*>(a.part_o + row * D + 16 * i + 4 * grp) = make_float4(r[0], r[1], r[2], r[3]);
+      else if constexpr (F32)
+        *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at + 16 * i) = make_float4(r[0], r[1], r[2], r[3]);
+      else
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at + 16 * i) = make_uint2(pack_half2(r[0], r[1]), pack_half2(r[2], r[3]));
     }
   }
 }

@@ -176,10 +176,12 @@ struct VTile<D, true> {
 template <int D, bool I4, bool F32>
 __global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) {
   constexpr int DT = D / 16, QT = D / 32, OS = D + 4;
-  // the queries' operands, and after the last tile the waves' outputs
+  // the queries' operands and which values were not finite; after the last tile the waves' outputs
   __shared__ __attribute__((aligned(16))) float smem[kWaves * 16 * OS];
-  static_assert(sizeof(smem) >= (F32 ? 2 : 1) * QT * 64 * sizeof(half8_t), "the queries fit");
+  constexpr int kQueries = (F32 ? 2 : 1) * QT * 64 * sizeof(half8_t);
+  static_assert(sizeof(smem) >= kQueries + kWaves * DT * 64 * sizeof(uint32_t), "both fit");
   half8_t(*q_s)[QT][64] = reinterpret_cast<half8_t(*)[QT][64]>(smem);
+  uint32_t(*seen_s)[DT][64] = reinterpret_cast<uint32_t(*)[DT][64]>(reinterpret_cast<char*>(smem) + kQueries);
   float(*o_s)[16][OS] = reinterpret_cast<float(*)[16][OS]>(smem);
   __shared__ float m_s[kWaves][16], l_s[kWaves][16];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -220,6 +222,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) 
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = float4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
+  bool seen = false;
   while (t < t_end) {
     const int tn = t + kWaves;
     float s[8];
@@ -239,11 +242,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) 
       for (int i = 0; i < 8; ++i) s[i] = sc[i >> 2][i & 3] * query.mult;
     }
     const Tile next = tile_of<kTile>(a, keys, tn < t_end ? tn : t);
+    const Sight sight = sight_of(a, keys, t, p);
     if (tn < t_end) kx.load(a, base, next, col, grp);
     if (!tile.whole) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (!sees(a, p, tile.key0 + 4 * grp + (i < 4 ? i : 12 + i), tile.end)) s[i] = -INFINITY;
+        if (!sight(tile.key0 + 4 * grp + (i < 4 ? i : 12 + i))) s[i] = -INFINITY;
     }
     float corr;
     const bool moves = soften(s, m, l, corr);
@@ -266,15 +270,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) 
         if constexpr (F32) o[i] = mfma(v, pl, o[i]);
       });
     } else {
-half8_t vis;
+      half8_t vis;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) vis[j] = sees(a, p, tile.key0 + 4 * grp + (j < 4 ? j : 12 + j), tile.end) ? (half_t)1.f : (half_t)0.f;
+      for (int j = 0; j < 8; ++j) vis[j] = sight(tile.key0 + 4 * grp + (j < 4 ? j : 12 + j)) ? (half_t)1.f : (half_t)0.f;
+      if (!seen) {
+#pragma unroll 1
+        for (int i = 0; i < DT; ++i) seen_s[wave][i][lane] = 0u;
+        seen = true;
+      }
       vx.each([&](int i, half8_t v) {
         half8_t mark;
         v = without_marked(v, mark);
         o[i] = mfma(v, ph, o[i]);
         if constexpr (F32) o[i] = mfma(v, pl, o[i]);
-        o[i] = with_seen(o[i], mfma(mark, vis, float4_t{0.f, 0.f, 0.f, 0.f}));
+        seen_s[wave][i][lane] |= seen_bits(mfma(mark, vis, float4_t{0.f, 0.f, 0.f, 0.f}));
+        __builtin_amdgcn_sched_barrier(0);
       });
     }
     if (tn < t_end) vx.load(a, base, next, col, grp);
@@ -284,6 +294,10 @@ half8_t vis;
 
   // merge the waves: outputs by column, then whole rows
   l = column_sum(l);
+  if (seen) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[i] = with_seen(o[i], seen_s[wave][i][lane]);
+  }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < DT; ++i)
