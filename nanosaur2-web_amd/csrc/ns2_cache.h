@@ -44,13 +44,12 @@ int launch_prompt(const AttnArgs& a, int D, hipStream_t s);
 // ---- 4-bit values ----------------------------------------------------------------------------
 
 // Four nibbles of each 16-bit half of x -> the half2 pairs (n0, n0'), (n1, n1') ...: 0x6400 | n is the half
-// 1024 + n, the subtraction is exact, and the fused multiply-add rounds offset + n * step once.
+// 1024 + n (and 0x6400 | 16 n is 1024 + 16 n), taking 1024 off (or a sixteenth, less 64) is exact, and the fused
+// multiply-add rounds offset + n * step once.
 __device__ __forceinline__ void dequant4(uint32_t x, half2_t s, half2_t o, uint32_t r[4]) {
+  nibbles4(x, half2_t{-1024.f, -1024.f}, half2_t{-64.f, -64.f}, r);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const half2_t n = __builtin_bit_cast(half2_t, ((x >> (4 * i)) & 0x000f000fu) | 0x64006400u) - half2_t{1024.f, 1024.f};
-    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, s, o));
-  }
+  for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2_t, r[i]), s, o));
 }
 
 // A word's eight values in the order 0 4 1 5 2 6 3 7 (operand elements; Q's are put in the same order).
@@ -161,6 +160,10 @@ __device__ __forceinline__ const char* tile_rows(const void* cache, long long ba
   return static_cast<const char*>(cache) + (i4 ? at / 2 : at * 2);
 }
 
+__device__ __forceinline__ const half2_t* tile_groups(const half2_t* groups, long long base, int key0, int ldkv) {
+  return groups + (base + (long long)key0 * ldkv) / kGroup;
+}
+
 // ---- queries -------------------------------------------------------------------------------------
 
 // Element e of operand step t of lane group grp is dimension qdim(t, grp) + e (fp16 cache: e in order, 4-bit:
@@ -171,53 +174,55 @@ __device__ __forceinline__ int qdim(int t, int grp) {
   return I4 ? grp * (D / 4) + 8 * t : 32 * t + 8 * grp;
 }
 
-// Column m's query, or null for padding (whose operands are zeros).
-template <bool F32>
+// Column m's query (zeros for padding). fp32 queries are scaled by a power of two to below 2^14 and taken as two
+// halves that keep 22 bits.
+template <int D, bool I4, bool F32>
 struct Query {
-  const char* at;
-  int up;      // fp32: scaled by 2^up, to below 2^14
-  float mult;  // what takes a score to a base-2 logarithm
+  static constexpr int QT = D / 32;
+  float4 x[F32 ? QT : 1][2];
+  half8_t h[F32 ? 1 : QT];
 
-  __device__ __forceinline__ float4 four(int d) const {
-    return at ? *reinterpret_cast<const float4*>(at + 4 * d) : make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  template <int D, bool I4>
-  __device__ __forceinline__ void open(const AttnArgs& a, int b, int g, int m, bool live, int grp) {
-    const int G = a.H / a.KH, i = live ? m / G : 0, h = live ? m - i * G : 0;
-    const long long e = ((long long)b * a.L + i) * a.ldq + (long long)(g * G + h) * D;
-    at = live ? static_cast<const char*>(a.q) + e * (F32 ? 4 : 2) : nullptr;
-    mult = a.scale;
-    up = 0;
-    if constexpr (F32) {
-      float top = 0.f;
+  __device__ __forceinline__ void load(const AttnArgs& a, int b, int g, int m, bool live, int grp) {
+    const int G = a.H / a.KH, i = live ? m / G : 0, hd = live ? m - i * G : 0;
+    const long long e = ((long long)b * a.L + i) * a.ldq + (long long)(g * G + hd) * D;
 #pragma unroll
-      for (int t = 0; t < D / 32; ++t) {
-        const float4 u = four(qdim<D, I4>(t, grp)), v = four(qdim<D, I4>(t, grp) + 4);
-        top = fmaxf(top, fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w))));
-        top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+    for (int t = 0; t < QT; ++t) {
+      const int d = qdim<D, I4>(t, grp);
+      if constexpr (F32) {
+        const float* q = static_cast<const float*>(a.q) + e + d;
+        x[t][0] = live ? *reinterpret_cast<const float4*>(q) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[t][1] = live ? *reinterpret_cast<const float4*>(q + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      } else {
+        h[t] = live ? *reinterpret_cast<const half8_t*>(static_cast<const half_t*>(a.q) + e + d) : half8_t{0, 0, 0, 0, 0, 0, 0, 0};
       }
-      top = column_max(top);
-      if (top > 0.f && top < INFINITY) up = min(14 - __builtin_amdgcn_frexp_expf(top), 120);
-      mult = ldexpf(a.scale, -up);
     }
   }
-  // The B operand of step t; PERM: in the order of dequant8. fp32: two halves that keep 22 bits.
-  template <int D, bool I4, bool PERM>
-  __device__ __forceinline__ void operand(int t, int grp, half8_t& hi, half8_t& lo) const {
-    constexpr int order[8] = {0, PERM ? 4 : 1, PERM ? 1 : 2, PERM ? 5 : 3, PERM ? 2 : 4, PERM ? 6 : 5, PERM ? 3 : 6, 7};
-    const int d = qdim<D, I4>(t, grp);
-    if constexpr (!F32) {
-      const half8_t x = at ? *reinterpret_cast<const half8_t*>(at + 2 * d) : half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+  // The exponent of the scaling, the same in the column's lanes.
+  __device__ __forceinline__ int up() const {
+    if constexpr (!F32) return 0;
+    float top = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) hi[e] = x[order[e]];
+    for (int t = 0; t < (F32 ? QT : 0); ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(x[t][i].x), fabsf(x[t][i].y)), fmaxf(fabsf(x[t][i].z), fabsf(x[t][i].w))));
+    top = column_max(top);
+    return top > 0.f && top < INFINITY ? min(14 - __builtin_amdgcn_frexp_expf(top), 120) : 0;
+  }
+  // The B operand of step t; PERM: in the order of dequant8.
+  template <bool PERM>
+  __device__ __forceinline__ void operand(int t, int up, half8_t& hi, half8_t& lo) const {
+    constexpr int order[8] = {0, PERM ? 4 : 1, PERM ? 1 : 2, PERM ? 5 : 3, PERM ? 2 : 4, PERM ? 6 : 5, PERM ? 3 : 6, 7};
+    if constexpr (!F32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) hi[e] = h[t][order[e]];
     } else {
-      const float4 u = four(d), v = four(d + 4);
-      const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+      const float y[8] = {x[t][0].x, x[t][0].y, x[t][0].z, x[t][0].w, x[t][1].x, x[t][1].y, x[t][1].z, x[t][1].w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float y = ldexpf(x[order[e]], up);
-        hi[e] = (half_t)y;
-        lo[e] = (half_t)(y - (float)hi[e]);
+        const float z = ldexpf(y[order[e]], up);
+        hi[e] = (half_t)z;
+        lo[e] = (half_t)(z - (float)hi[e]);
       }
     }
   }
@@ -256,13 +261,16 @@ __device__ __forceinline__ bool soften(float (&s)[N], float& m, float& l, float&
 __device__ __forceinline__ float4_t mfma(half8_t a, half8_t b, float4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ float4_t mfma(half4_t a, half4_t b, float4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+}
 
 // The B operand of the second product: eight weights, rounded to halves, or (F32) as two halves: the leading
 // 11 bits and the rest, which keeps 21 to 22 bits in all.
-template <bool F32>
-__device__ __forceinline__ void weights(const float* p, half8_t& hi, half8_t& lo) {
+template <bool F32, int N, class H>
+__device__ __forceinline__ void weights(const float (&p)[N], H& hi, H& lo) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < N; ++e) {
     if constexpr (!F32) {
       hi[e] = (half_t)p[e];
     } else {
@@ -277,9 +285,10 @@ __device__ __forceinline__ void weights(const float* p, half8_t& hi, half8_t& lo
 // taken out of the product, and a second product of marks (1 for inf, 64 for -inf, 4096 for NaN) with the
 // columns' visible keys (1 or 0) tells each output what it has seen (at most 32 of each per product). What was
 // seen is kept aside, one byte per output, and put into the outputs at the end.
-__device__ __forceinline__ half8_t without_marked(half8_t v, half8_t& mark) {
+template <class H>
+__device__ __forceinline__ H without_marked(H v, H& mark) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < (int)(sizeof(H) / 2); ++e) {
     const half_t x = v[e];  // (a bit cast of the element itself would read element 0)
     const uint16_t u = __builtin_bit_cast(uint16_t, x), size = u & 0x7fffu;
     mark[e] = size < 0x7c00u ? (half_t)0.f : size > 0x7c00u ? (half_t)4096.f : u == size ? (half_t)1.f : (half_t)64.f;
@@ -307,13 +316,20 @@ __device__ __forceinline__ float4_t with_seen(float4_t o, uint32_t bits) {
 }
 
 // Adds 0 * v: NaN once v held an infinity or a NaN.
+__device__ __forceinline__ void spot(uint32_t v, half2_t& z) {
+  z = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, v), half2_t{0.f, 0.f}, z);
+}
+__device__ __forceinline__ void spot(half4_t v, half2_t& z) {
+  const uint2 w = __builtin_bit_cast(uint2, v);
+  spot(w.x, z);
+  spot(w.y, z);
+}
 __device__ __forceinline__ void spot(half8_t v, half2_t& z) {
   const uint4 w = __builtin_bit_cast(uint4, v);
-  const half2_t zero = {0.f, 0.f};
-  z = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, w.x), zero, z);
-  z = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, w.y), zero, z);
-  z = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, w.z), zero, z);
-  z = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, w.w), zero, z);
+  spot(w.x, z);
+  spot(w.y, z);
+  spot(w.z, z);
+  spot(w.w, z);
 }
 
 }  // namespace ns2cache

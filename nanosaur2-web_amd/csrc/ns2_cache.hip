@@ -130,8 +130,8 @@ __global__ __launch_bounds__(256) void cache_write_kernel(WriteArgs a) {
 // ---- attention: the splits joined, and which kernel runs ---------------------------------------------
 
 // One block per column: the splits' sums weighted to their common maximum. D / 4 lanes hold a row of D, so that
-// the block's Z groups of lanes take a split each, up to four at a time in flight; the groups are added in order.
-// A split that saw no key has maximum -inf and its sums are not taken.
+// the block's Z groups of lanes take a split each, four at a time in flight; the groups are added in order. What a
+// split that saw no key (maximum -inf, sum 0) left as its sums is not taken.
 constexpr int kMaxSplits = 64;
 
 template <int D>
@@ -143,37 +143,40 @@ __global__ __launch_bounds__(256) void cache_join_kernel(AttnArgs a) {
   const int G = a.H / a.KH, R = a.L * G;
   const long long columns = (long long)a.batch * a.KH * R, u = blockIdx.x;
   const int bg = (int)(u / R), mc = (int)(u - (long long)bg * R), b = bg / a.KH, g = bg - b * a.KH;
-  if (column_pos(a, b, mc) < 0) return;
+  // everything is asked for at once: the column's position, the splits' statistics and their first sums
+  const int p = column_pos(a, b, mc);
   const float2 ml = lane < a.splits ? a.part_s[lane * columns + u] : make_float2(-INFINITY, 0.f);
+  const int sub = lane / T, t = lane - sub * T, zg = wave * PW + sub;
+  float4 x[4];
+  auto load = [&](int z0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = sub < PW && z0 + i * Z < a.splits ? *reinterpret_cast<const float4*>(a.part_o + ((z0 + i * Z) * columns + u) * D + 4 * t)
+                                               : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  load(zg);
+  if (p < 0) return;
   float top = ml.x;
   for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
   const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
   const float sum = wave_sum(f * ml.y);
   if (wave == 0) f_s[lane] = ml.x == -INFINITY && ml.y == 0.f ? -1.f : f;
   __syncthreads();
-  const int sub = lane / T, t = lane - sub * T, zg = wave * PW + sub;
   float r[4] = {0.f, 0.f, 0.f, 0.f};
-  if (sub < PW) {
-    for (int z0 = zg; z0 < a.splits; z0 += 4 * Z) {
-      float4 x[4];
+  for (int z0 = zg; z0 < a.splits; z0 += 4 * Z) {
+    if (z0 != zg) load(z0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int z = z0 + i * Z;
-        if (z < a.splits && f_s[z] >= 0.f) x[i] = *reinterpret_cast<const float4*>(a.part_o + (z * columns + u) * D + 4 * t);
-        else x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int z = z0 + i * Z;
-        const float w = z < a.splits && f_s[z] >= 0.f ? f_s[z] : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      const float w = z0 + i * Z < a.splits ? f_s[z0 + i * Z] : -1.f;
+      if (w >= 0.f || w != w) {
         r[0] += w * x[i].x;
         r[1] += w * x[i].y;
         r[2] += w * x[i].z;
         r[3] += w * x[i].w;
       }
     }
-    o_s[zg][t] = make_float4(r[0], r[1], r[2], r[3]);
   }
+  if (sub < PW) o_s[zg][t] = make_float4(r[0], r[1], r[2], r[3]);
   __syncthreads();
   if (threadIdx.x >= T) return;
   float4 q = o_s[0][t];
@@ -205,8 +208,8 @@ Plan plan_of(int batch, int L, int H, int KH, int cap, int window, int sinks) {
   p.prompt = R > kRowsColumns;
   const long long blocks = heads * (p.prompt ? (R + 63) / 64 : (R + 15) / 16);
   const long long want = p.prompt ? kCUs / blocks : 2 * kCUs / blocks;
-  // at least four tiles of 64 keys, or two of 32 for each of four waves, per split
-  const long long most = std::min<long long>(kMaxSplits, std::max<long long>(1, keys / 256));
+  // at least 64 keys per split
+  const long long most = std::min<long long>(kMaxSplits, std::max<long long>(1, keys / 64));
   p.splits = (int)std::max<long long>(1, std::min(want, most));
   return p;
 }

@@ -31,6 +31,7 @@ struct Stage {
 
   __device__ __forceinline__ void load_k(const AttnArgs& a, long long base, const Tile& t, int tid) {
     const char* rows = tile_rows(a.k, base, t.key0, a.ldkv, I4);
+    const half2_t* groups = I4 ? tile_groups(a.kg, base, t.key0, a.ldkv) : nullptr;
     const int last = t.end - 1 - t.key0;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
@@ -38,7 +39,7 @@ struct Stage {
       const uint32_t at = (uint32_t)(key * a.ldkv + 8 * c);
       if constexpr (I4) {
         raw[i] = *reinterpret_cast<const uint32_t*>(rows + at / 2);
-        group[i] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(a.kg) + (base + (long long)t.key0 * a.ldkv) / kGroup * 4 + at / kGroup * 4);
+        group[i] = __builtin_bit_cast(uint32_t, groups[at / kGroup]);
       } else {
         const uint4 x = *reinterpret_cast<const uint4*>(rows + 2u * at);
         raw[4 * i] = x.x;
@@ -52,6 +53,7 @@ struct Stage {
   __device__ __forceinline__ void load_v(const AttnArgs& a, long long base, const Tile& t, int tid) {
     if (8 * VC < kHalf && tid >= 8 * VC) return;
     const char* rows = tile_rows(a.v, base, t.key0, a.ldkv, I4);
+    const half2_t* groups = I4 ? tile_groups(a.vg, base, t.key0, a.ldkv) : nullptr;
     const int last = t.end - 1 - t.key0;
     const int c = tid % VC, q = tid / VC;  // q = 4 (tile half) + lane group
 #pragma unroll
@@ -62,7 +64,7 @@ struct Stage {
         raw[j] = VD == 8   ? *reinterpret_cast<const uint32_t*>(rows + at / 2)
                  : VD == 4 ? *reinterpret_cast<const uint16_t*>(rows + at / 2)
                            : *reinterpret_cast<const uint8_t*>(rows + at / 2);
-        group[j] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(a.vg) + (base + (long long)t.key0 * a.ldkv) / kGroup * 4 + at / kGroup * 4);
+        group[j] = __builtin_bit_cast(uint32_t, groups[at / kGroup]);
       } else if constexpr (VD == 8) {
         const uint4 x = *reinterpret_cast<const uint4*>(rows + 2u * at);
         raw[4 * j] = x.x;
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
   __shared__ uint32_t seen_s[8][CT * DT][64];  // values that were not finite
   __shared__ int bad_s;                        // 1 + the last tile with such a V value
   half8_t *k_s = smem, *v_s = smem + 4 * QT * 64;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int half = wave >> 2, tid = threadIdx.x & (kHalf - 1);  // waves 0-3: first half of a tile, bring K
   const int col = lane & 15, grp = lane >> 4;
   const int G = a.H / a.KH, R = a.L * G;
@@ -181,11 +183,12 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
   for (int c = 0; c < CT; ++c) {
     const int mc = m0 + ((wave & 3) * CT + c) * 16 + col;
     p[c] = column_pos(a, b, mc);
-    Query<F32> query;
-    query.template open<D, false>(a, b, g, mc, p[c] >= 0, grp);
-    mult[c] = query.mult;
+    Query<D, false, F32> query;
+    query.load(a, b, g, mc, p[c] >= 0, grp);
+    const int up = query.up();
+    mult[c] = ldexpf(a.scale, -up);
 #pragma unroll
-    for (int i = 0; i < QT; ++i) query.template operand<D, false, I4>(i, grp, qh[c][i], ql[c][F32 ? i : 0]);
+    for (int i = 0; i < QT; ++i) query.template operand<I4>(i, up, qh[c][i], ql[c][F32 ? i : 0]);
     m[c] = -INFINITY;
     l[c] = 0.f;
 #pragma unroll

@@ -284,6 +284,28 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   return __builtin_bit_cast(uint32_t, h);
 }
 
+// ---- 4-bit codes ------------------------------------------------------------------------------
+// The four nibbles n of each 16-bit half of x as half2 pairs, (n0, n0') first, each plus `even` + 1024 (nibbles
+// 0 and 2) or `odd` + 64 (1 and 3): 0x6400 | n is the half 1024 + n, 0x6400 | 16 n the half 1024 + 16 n, and both
+// steps are exact for sums that are small integers. The mask is one instruction with the or (v_and_or_b32
+// takes one scalar operand: the mask; the compiler would split it in two with literals).
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "s"(mask), "v"(bits));
+  return r;
+}
+__device__ __forceinline__ void nibbles4(uint32_t x, half2_t even, half2_t odd, uint32_t r[4]) {
+  const half2_t sixteenth = {0.0625f, 0.0625f};
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const uint32_t y = i ? x >> 8 : x;
+    const half2_t a = __builtin_bit_cast(half2_t, and_or(y, 0x000f000fu, 0x64006400u));
+    const half2_t b = __builtin_bit_cast(half2_t, and_or(y, 0x00f000f0u, 0x64006400u));
+    r[i] = __builtin_bit_cast(uint32_t, a + even);
+    r[i + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, sixteenth, odd));
+  }
+}
+
 // Offset (in halfs) of element (m, k) of an fp16 GEMM operand with K columns in the tiled
 // layout of the int8 GEMM: [M/64][K/64][8 k-chunks][64 rows][8 halfs] (ns2_linear_i8_tiled).
 __device__ __forceinline__ long long tiled_off(long long m, int k, int K) {

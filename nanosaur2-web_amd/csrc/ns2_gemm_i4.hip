@@ -69,12 +69,10 @@ __device__ __forceinline__ void transpose_rows(uint32_t w[4]) {
   swap16(w[2], w[3]);
 }
 
-// code - 8 of a word's eight codes: 0x6400 | c is the half 1024 + c.
+// code - 8 of a word's eight codes
 __device__ __forceinline__ half8_t codes8(uint32_t w) {
   uint32_t r[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - half2_t{1032.f, 1032.f});
+  nibbles4(w, half2_t{-1032.f, -1032.f}, half2_t{-72.f, -72.f}, r);
   return __builtin_bit_cast(half8_t, make_uint4(r[0], r[1], r[2], r[3]));
 }
 
@@ -91,7 +89,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear_i4_kernel(I4Args p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   half8_t* x_s = reinterpret_cast<half8_t*>(smem);
   __shared__ uint32_t top_s[16 * RT];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c16 = lane & 15, g = lane >> 4;
   const int m0 = blockIdx.y * (16 * RT);
   const int rows = p.M - m0 < 16 * RT ? p.M - m0 : 16 * RT;
