@@ -284,7 +284,7 @@ __device__ __forceinline__ void weights(const float (&p)[N], H& hi, H& lo) {
 // Values that are not finite must reach the columns that see them and no others, but 0 * inf is NaN: they are
 // taken out of the product, and a second product of marks (1 for inf, 64 for -inf, 4096 for NaN) with the
 // columns' visible keys (1 or 0) tells each output what it has seen (at most 32 of each per product). What was
-// seen is kept aside, one byte per output, and put into the outputs at the end.
+// seen is kept aside and put into the outputs at the end.
 template <class H>
 __device__ __forceinline__ H without_marked(H v, H& mark) {
 #pragma unroll
@@ -296,20 +296,20 @@ __device__ __forceinline__ H without_marked(H v, H& mark) {
   }
   return v;
 }
-// bits per output: 1 inf, 2 -inf, 4 NaN
+// Two bits per output: 1 inf, 2 -inf, 3 NaN (and what both infinities add up to).
 __device__ __forceinline__ uint32_t seen_bits(float4_t count) {
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = (int)count[i];
-    w |= (uint32_t)((c & 63 ? 1 : 0) | (c & 0xfc0 ? 2 : 0) | (c >= 4096 ? 4 : 0)) << (8 * i);
+    w |= (uint32_t)((c & 63 ? 1 : 0) | (c & 0xfc0 ? 2 : 0) | (c >= 4096 ? 3 : 0)) << (2 * i);
   }
   return w;
 }
 __device__ __forceinline__ float4_t with_seen(float4_t o, uint32_t bits) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t b = (bits >> (8 * i)) & 7u;
+    const uint32_t b = (bits >> (2 * i)) & 3u;
     if (b) o[i] += b == 1 ? INFINITY : b == 2 ? -INFINITY : NAN;
   }
   return o;

@@ -137,17 +137,25 @@ template <int D, bool I4, bool F32, int CT>
 __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
   constexpr int DT = D / 16, QT = D / 32, VD = Stage<D, I4>::VD;
   constexpr int kFrags = 4 * QT + 2 * DT, kMerge = 4 * CT * (DT + 1);  // KB of a tile; of the second halves' sums
-  __shared__ __attribute__((aligned(16))) half8_t smem[(kFrags > kMerge ? kFrags : kMerge) * 64];
-  __shared__ uint32_t seen_s[8][CT * DT][64];  // values that were not finite
-  __shared__ int bad_s;                        // 1 + the last tile with such a V value
-  half8_t *k_s = smem, *v_s = smem + 4 * QT * 64;
+  __shared__ __attribute__((aligned(16))) half8_t smem[(2 * kFrags > kMerge ? 2 * kFrags : kMerge) * 64];
+  __shared__ uint8_t seen_s[8][CT * DT][64];  // values that were not finite
+  __shared__ int bad_s[2];                    // 1 + the last tile in this buffer with such a V value
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int half = wave >> 2, tid = threadIdx.x & (kHalf - 1);  // waves 0-3: first half of a tile, bring K
   const int col = lane & 15, grp = lane >> 4;
   const int G = a.H / a.KH, R = a.L * G;
-  const int z = blockIdx.x % a.splits, bg = blockIdx.x / a.splits;
+  // Blocks go to the eight dies in turn. Where all of a sequence is visible, its columns with the most keys go
+  // first; in a window, where neighbours share keys, each die takes a run of columns.
+  int by = gridDim.y - 1 - blockIdx.y, bx = blockIdx.x;
+  if (a.window) {
+    const int n = gridDim.x * gridDim.y, id = blockIdx.x + gridDim.x * blockIdx.y, even = n / 8, odd = n - 8 * even;
+    const int die = id & 7, at = die * even + min(die, odd) + (id >> 3);
+    bx = at / gridDim.y;
+    by = at - bx * gridDim.y;
+  }
+  const int z = bx % a.splits, bg = bx / a.splits;
   const int b = bg / a.KH, g = bg - b * a.KH;
-  const int m0 = (gridDim.y - 1 - blockIdx.y) * (64 * CT);  // the columns with the most keys first
+  const int m0 = by * (64 * CT);
 
   // the block's first and last position
   int hi_p = -1, lo_p = INT32_MAX;
@@ -170,11 +178,19 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
   const long long base = (long long)b * a.kvBatch + (long long)g * D;
 
   Stage<D, I4> st;
+  // (The two ends differ so that the compiler does not join the branches' last loads into one whose register
+  // is an index, which would put them into memory.)
+  auto load = [&](const Tile& tl) {
+    if (half == 0) {
+      st.load_k(a, base, tl, tid);
+      asm volatile("; K rows");
+    } else {
+      st.load_v(a, base, tl, tid);
+      asm volatile("; V rows");
+    }
+  };
   Tile tile = tile_of<kTile>(a, keys, t0 < t1 ? t0 : 0);
-  if (t0 < t1) {
-    if (half == 0) st.load_k(a, base, tile, tid);
-    else st.load_v(a, base, tile, tid);
-  }
+  if (t0 < t1) load(tile);
   half8_t qh[CT][QT], ql[CT][F32 ? QT : 1];
   float mult[CT], m[CT], l[CT];
   int p[CT];
@@ -194,24 +210,27 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[c][i] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
-  if (threadIdx.x == 0) bad_s = 0;
   bool seen = false;
-
-  for (int t = t0; t < t1; ++t) {
-    __syncthreads();  // the last tile's fragments are used
+  // tile t + 1's fragments are written while tile t's are used: one barrier per tile
+  auto store = [&](int t, const Tile& tl) {
+    half8_t* k_s = smem + ((t - t0) & 1) * (kFrags * 64);
     if (half == 0) {
       st.store_k(k_s, tid);
     } else {
-      const half2_t zz = st.store_v(v_s, tid, !tile.whole);
-      if (!(zz[0] == 0.f && zz[1] == 0.f)) bad_s = t + 1;
+      const half2_t zz = st.store_v(k_s + 4 * QT * 64, tid, !tl.whole);
+      if (!(zz[0] == 0.f && zz[1] == 0.f)) bad_s[(t - t0) & 1] = t + 1;
     }
-    __syncthreads();
-    const Tile next = tile_of<kTile>(a, keys, t + 1 < t1 ? t + 1 : t);
-    if (t + 1 < t1) {
-      if (half == 0) st.load_k(a, base, next, tid);
-      else st.load_v(a, base, next, tid);
-    }
+  };
+  if (threadIdx.x < 2) bad_s[threadIdx.x] = 0;
+  __syncthreads();
+  Tile next = tile_of<kTile>(a, keys, t0 + 1 < t1 ? t0 + 1 : t0);
+  if (t0 < t1) store(t0, tile);
+  if (t0 + 1 < t1) load(next);
+  __syncthreads();
 
+  for (int t = t0; t < t1; ++t) {
+    const half8_t* k_s = smem + ((t - t0) & 1) * (kFrags * 64);
+    half8_t* v_s = smem + ((t - t0) & 1) * (kFrags * 64) + 4 * QT * 64;
     float4_t s[CT][2];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
@@ -228,6 +247,11 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
           if constexpr (F32) s[c][kt] = mfma(k8, ql[c][i], s[c][kt]);
         }
       }
+    const Tile after = tile_of<kTile>(a, keys, t + 2 < t1 ? t + 2 : t);
+    if (t + 1 < t1) {
+      store(t + 1, next);
+      if (t + 2 < t1) load(after);
+    }
     half8_t ph[CT], pl[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -248,7 +272,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
       }
       weights<F32>(w, ph[c], pl[c]);
     }
-    if (!tile.whole && bad_s == t + 1) {  // (for all waves)
+    if (!tile.whole && bad_s[(t - t0) & 1] == t + 1) {  // (for all waves)
       half8_t vis[CT];
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
@@ -263,8 +287,8 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
         without_marked(v_s[(i * 2 + half) * 64 + grp * 16 + (col ^ (i & (VD - 1)))], mark);
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-          uint32_t* w = &seen_s[wave][c * DT + i][lane];
-          *w = (seen ? *w : 0u) | seen_bits(mfma(mark, vis[c], float4_t{0.f, 0.f, 0.f, 0.f}));
+          uint8_t* w = &seen_s[wave][c * DT + i][lane];
+          *w = (seen ? *w : 0) | seen_bits(mfma(mark, vis[c], float4_t{0.f, 0.f, 0.f, 0.f}));
         }
       }
       seen = true;
@@ -286,6 +310,8 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
       }
     }
     tile = next;
+    next = after;
+    __syncthreads();
   }
 
   if (seen) {
@@ -298,7 +324,6 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
   // the second halves' sums through LDS to the first's
   float4_t* o_s = reinterpret_cast<float4_t*>(smem) + (wave & 3) * (CT * DT * 64);
   float2* ml_s = reinterpret_cast<float2*>(reinterpret_cast<float4_t*>(smem) + 4 * CT * DT * 64) + (wave & 3) * (CT * 64);
-  __syncthreads();
   if (half) {
 #pragma unroll
     for (int c = 0; c < CT; ++c) {

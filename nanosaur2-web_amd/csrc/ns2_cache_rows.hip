@@ -190,9 +190,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) 
   // the queries' operands and which values were not finite; after the last tile the waves' outputs
   __shared__ __attribute__((aligned(16))) float smem[kWaves * 16 * OS];
   constexpr int kQueries = (F32 ? 2 : 1) * QT * 64 * sizeof(half8_t);
-  static_assert(sizeof(smem) >= kQueries + kWaves * DT * 64 * sizeof(uint32_t), "both fit");
+  static_assert(sizeof(smem) >= kQueries + kWaves * DT * 64, "both fit");
   half8_t(*q_s)[QT][64] = reinterpret_cast<half8_t(*)[QT][64]>(smem);
-  uint32_t(*seen_s)[DT][64] = reinterpret_cast<uint32_t(*)[DT][64]>(reinterpret_cast<char*>(smem) + kQueries);
+  uint8_t(*seen_s)[DT][64] = reinterpret_cast<uint8_t(*)[DT][64]>(reinterpret_cast<char*>(smem) + kQueries);
   float(*o_s)[16][OS] = reinterpret_cast<float(*)[16][OS]>(smem);
   __shared__ float m_s[kWaves][16], l_s[kWaves][16];
   __shared__ int p_s[16];
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) 
       for (int j = 0; j < NK; ++j) vis[j] = sight(tile.key0 + key_of(grp, j)) ? (half_t)1.f : (half_t)0.f;
       if (!seen) {
 #pragma unroll 1
-        for (int i = 0; i < DT; ++i) seen_s[wave][i][lane] = 0u;
+        for (int i = 0; i < DT; ++i) seen_s[wave][i][lane] = 0;
         seen = true;
       }
       vx.each([&](int i, Part v) {

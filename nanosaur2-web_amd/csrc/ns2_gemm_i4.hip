@@ -104,20 +104,19 @@ __global__ __launch_bounds__(64 * kWaves) void linear_i4_kernel(I4Args p) {
     wr[c] = p.W + (long long)n * kb;
     sr[c] = p.scale + (long long)n * kg;
   }
-  uint4 w[CT];
-  half_t sc[CT];
-  auto load = [&](int chunk) {
+  // the wave's next PD chunks are on their way
+  constexpr int PD = RT > 2 ? 1 : CT == 1 ? 4 : 2;
+  uint4 w[PD][CT];
+  half_t sc[PD][CT];
+  auto load = [&](int s, int chunk) {
     int k = chunk * kChunk + 32 * g;
     k = k < p.K ? k : 0;  // (a step past K is not used)
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      w[c] = *reinterpret_cast<const uint4*>(wr[c] + k / 2);
-      sc[c] = sr[c][k / (32 * SG)];
+      w[s][c] = *reinterpret_cast<const uint4*>(wr[c] + k / 2);
+      sc[s][c] = sr[c][k / (32 * SG)];
     }
   };
-  const int chunks = (p.K + kChunk - 1) / kChunk;
-  int chunk = WK == 1 ? 0 : wave;
-  if (chunk < chunks) load(chunk);
 
   float tot[RT][CT][NR];
 #pragma unroll
@@ -139,6 +138,10 @@ __global__ __launch_bounds__(64 * kWaves) void linear_i4_kernel(I4Args p) {
     const int ks = p.K - k0 < p.slab ? p.K - k0 : p.slab;
     const int n8 = ks / 8, items = rows * n8;
     half8_t* lo_s = x_s + items;
+    const int first = k0 / kChunk + (WK == 1 ? 0 : wave), last = (k0 + ks + kChunk - 1) / kChunk;
+#pragma unroll
+    for (int s = 0; s < PD; ++s)
+      if (first + s * WK < last) load(s, first + s * WK);
     if (k0) __syncthreads();  // the last slab is used
     if constexpr (A16) {
       for (int u = threadIdx.x; u < items; u += 64 * kWaves) {
@@ -147,32 +150,49 @@ __global__ __launch_bounds__(64 * kWaves) void linear_i4_kernel(I4Args p) {
         x_s[k8 * rows + r] = half8_t{x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
       }
     } else {
+      constexpr int NI = kSlabBytes / 32 / (64 * kWaves);  // pieces of 8 columns per thread
+      float4 y[NI][2];
+      float top[NI];
       for (int u = threadIdx.x; u < rows; u += 64 * kWaves) top_s[u] = 0u;
-      __syncthreads();
-      for (int u = threadIdx.x; u < items; u += 64 * kWaves) {
-        const int r = u / n8, k8 = u - r * n8;
-        const float* a = static_cast<const float*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8;
-        const float4 y = *reinterpret_cast<const float4*>(a), z = *reinterpret_cast<const float4*>(a + 4);
-        const float top = fmaxf(fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))),
-                                fmaxf(fmaxf(fabsf(z.x), fabsf(z.y)), fmaxf(fabsf(z.z), fabsf(z.w))));
-        atomicMax(&top_s[r], __builtin_bit_cast(uint32_t, top));  // magnitudes order as their bits do
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int u = threadIdx.x + 64 * kWaves * i, r = u / n8, k8 = u - r * n8;
+        y[i][0] = y[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (u < items) {
+          const float* a = static_cast<const float*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8;
+          y[i][0] = *reinterpret_cast<const float4*>(a);
+          y[i][1] = *reinterpret_cast<const float4*>(a + 4);
+        }
       }
       __syncthreads();
-      for (int u = threadIdx.x; u < items; u += 64 * kWaves) {
-        const int r = u / n8, k8 = u - r * n8;
-        const float* a = static_cast<const float*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8;
-        const float4 y = *reinterpret_cast<const float4*>(a), z = *reinterpret_cast<const float4*>(a + 4);
-        const float v[8] = {y.x, z.x, y.y, z.y, y.z, z.z, y.w, z.w};
-        const int up = i4_up(__builtin_bit_cast(float, top_s[r]));
-        half8_t hi, lo;
+      // magnitudes order as their bits do; four neighbours share a row (n8 is a multiple of 4)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float t = ldexpf(v[e], up);
-          hi[e] = (half_t)t;
-          lo[e] = (half_t)(t - (float)hi[e]);
+      for (int i = 0; i < NI; ++i) {
+        const int u = threadIdx.x + 64 * kWaves * i;
+        const float4 a = y[i][0], b = y[i][1];
+        top[i] = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
+                       fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
+        top[i] = fmaxf(top[i], dpp<kDppXor1>(top[i]));
+        top[i] = fmaxf(top[i], dpp<kDppXor2>(top[i]));
+        if (u < items && (threadIdx.x & 3) == 0) atomicMax(&top_s[u / n8], __builtin_bit_cast(uint32_t, top[i]));
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int u = threadIdx.x + 64 * kWaves * i, r = u / n8, k8 = u - r * n8;
+        if (u < items) {
+          const float v[8] = {y[i][0].x, y[i][1].x, y[i][0].y, y[i][1].y, y[i][0].z, y[i][1].z, y[i][0].w, y[i][1].w};
+          const int up = i4_up(__builtin_bit_cast(float, top_s[r]));
+          half8_t hi, lo;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float t = ldexpf(v[e], up);
+            hi[e] = (half_t)t;
+            lo[e] = (half_t)(t - (float)hi[e]);
+          }
+          x_s[k8 * rows + r] = hi;
+          lo_s[k8 * rows + r] = lo;
         }
-        x_s[k8 * rows + r] = hi;
-        lo_s[k8 * rows + r] = lo;
       }
     }
     __syncthreads();
@@ -184,52 +204,57 @@ __global__ __launch_bounds__(64 * kWaves) void linear_i4_kernel(I4Args p) {
       for (int c = 0; c < CT; ++c)
 #pragma unroll
         for (int r = 0; r < NR; ++r) acc[i][c][r] = 0.f;
-    const int last = (k0 + ks + kChunk - 1) / kChunk;
-    for (; chunk < last; chunk += WK) {
-      uint32_t t[CT][4];
-      float s[CT][4];
+    for (int chunk = first; chunk < last; chunk += PD * WK) {
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        t[c][0] = w[c].x;
-        t[c][1] = w[c].y;
-        t[c][2] = w[c].z;
-        t[c][3] = w[c].w;
-        const float f = (float)sc[c];
-        uint32_t a = __builtin_bit_cast(uint32_t, f), b = a;
-        swap32(a, b);  // the scales of steps 0, 1 | 2, 3
-        uint32_t a1 = a, b1 = b;
-        swap16(a, a1);
-        swap16(b, b1);
-        s[c][0] = __builtin_bit_cast(float, a);
-        s[c][1] = __builtin_bit_cast(float, a1);
-        s[c][2] = __builtin_bit_cast(float, b);
-        s[c][3] = __builtin_bit_cast(float, b1);
-      }
-      if (chunk + WK < chunks) load(chunk + WK);
-#pragma unroll
-      for (int c = 0; c < CT; ++c) transpose_rows(t[c]);
-      const int base = (chunk * kChunk - k0) / 8 + g;
-      float4_t d[RT][CT];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (chunk * kChunk + 32 * j < k0 + ks) {  // uniform
-          half8_t xh[RT], xl[RT];
-#pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            xh[i] = x_s[(base + 4 * j) * rows + arow[i]];
-            if constexpr (!A16) xl[i] = lo_s[(base + 4 * j) * rows + arow[i]];
-          }
+      for (int sl = 0; sl < PD; ++sl) {
+        const int ch = chunk + sl * WK;
+        if (ch < last) {  // uniform
+          uint32_t t[CT][4];
+          float s[CT][4];
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
-            const half8_t q = codes8(t[c][j]);
+            t[c][0] = w[sl][c].x;
+            t[c][1] = w[sl][c].y;
+            t[c][2] = w[sl][c].z;
+            t[c][3] = w[sl][c].w;
+            const float f = (float)sc[sl][c];
+            uint32_t a = __builtin_bit_cast(uint32_t, f), b = a;
+            swap32(a, b);  // the scales of steps 0, 1 | 2, 3
+            uint32_t a1 = a, b1 = b;
+            swap16(a, a1);
+            swap16(b, b1);
+            s[c][0] = __builtin_bit_cast(float, a);
+            s[c][1] = __builtin_bit_cast(float, a1);
+            s[c][2] = __builtin_bit_cast(float, b);
+            s[c][3] = __builtin_bit_cast(float, b1);
+          }
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-              if (j % SG == 0) d[i][c] = float4_t{0.f, 0.f, 0.f, 0.f};
-              d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[i], q, d[i][c], 0, 0, 0);
-              if constexpr (!A16) d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[i], q, d[i][c], 0, 0, 0);
-              if (j % SG == SG - 1) {
+          for (int c = 0; c < CT; ++c) transpose_rows(t[c]);
+          if (ch + PD * WK < last) load(sl, ch + PD * WK);
+          const int base = (ch * kChunk - k0) / 8 + g;
+          float4_t d[RT][CT];
 #pragma unroll
-                for (int r = 0; r < NR; ++r) acc[i][c][r] = fmaf(s[c][j], d[i][c][r], acc[i][c][r]);
+          for (int j = 0; j < 4; ++j) {
+            if (ch * kChunk + 32 * j < k0 + ks) {  // uniform
+              half8_t xh[RT], xl[RT];
+#pragma unroll
+              for (int i = 0; i < RT; ++i) {
+                xh[i] = x_s[(base + 4 * j) * rows + arow[i]];
+                if constexpr (!A16) xl[i] = lo_s[(base + 4 * j) * rows + arow[i]];
+              }
+#pragma unroll
+              for (int c = 0; c < CT; ++c) {
+                const half8_t q = codes8(t[c][j]);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                  if (j % SG == 0) d[i][c] = float4_t{0.f, 0.f, 0.f, 0.f};
+                  d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[i], q, d[i][c], 0, 0, 0);
+                  if constexpr (!A16) d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[i], q, d[i][c], 0, 0, 0);
+                  if (j % SG == SG - 1) {
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) acc[i][c][r] = fmaf(s[c][j], d[i][c][r], acc[i][c][r]);
+                  }
+                }
               }
             }
           }
