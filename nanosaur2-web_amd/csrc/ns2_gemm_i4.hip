@@ -76,16 +76,24 @@ __device__ __forceinline__ half8_t codes8(uint32_t w) {
   return __builtin_bit_cast(half8_t, make_uint4(r[0], r[1], r[2], r[3]));
 }
 
-constexpr int kWaves = 4;
-constexpr int kChunk = 128;            // columns of k per load
-constexpr int kSlabBytes = 48 * 1024;  // LDS for the rows of x
+constexpr int kChunk = 128;  // columns of k per load
+// Waves of a block, and its LDS for the rows of x.
+template <int WK>
+constexpr int waves() {
+  return WK == 16 ? 16 : 4;
+}
+template <bool A16, int RT>
+constexpr int slab_bytes() {
+  return A16 && RT > 1 ? 32 * 1024 : 48 * 1024;
+}
 
 // A block takes 16 RT rows and, with WK = 1, 64 CT columns (16 CT per wave) over all of K; with WK = 4, 16 CT
 // columns whose chunks its waves take in turn and add up at the end. NR: result registers in use (4 NR rows of
 // each 16). SG: 32-column steps per group. The block's rows of x go to LDS a slab of p.slab columns at a time:
 // operand (step, lane group, row), `rows` rows, hi then lo.
 template <bool A16, int SG, int RT, int NR, int CT, int WK>
-__global__ __launch_bounds__(64 * kWaves) void linear_i4_kernel(I4Args p) {
+__global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p) {
+  constexpr int kWaves = waves<WK>();
   extern __shared__ __attribute__((aligned(16))) char smem[];
   half8_t* x_s = reinterpret_cast<half8_t*>(smem);
   __shared__ uint32_t top_s[16 * RT];
@@ -105,7 +113,7 @@ __global__ __launch_bounds__(64 * kWaves) void linear_i4_kernel(I4Args p) {
     sr[c] = p.scale + (long long)n * kg;
   }
   // the wave's next PD chunks are on their way
-  constexpr int PD = RT > 2 ? 1 : CT == 1 ? 4 : 2;
+  constexpr int PD = CT == 1 ? 4 : 2;
   uint4 w[PD][CT];
   half_t sc[PD][CT];
   auto load = [&](int s, int chunk) {
@@ -146,22 +154,21 @@ __global__ __launch_bounds__(64 * kWaves) void linear_i4_kernel(I4Args p) {
     if constexpr (A16) {
       for (int u = threadIdx.x; u < items; u += 64 * kWaves) {
         const int r = u / n8, k8 = u - r * n8;
-        const half8_t x = *reinterpret_cast<const half8_t*>(static_cast<const half_t*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8);
-        x_s[k8 * rows + r] = half8_t{x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
+        const half8_t v = *reinterpret_cast<const half8_t*>(static_cast<const half_t*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8);
+        x_s[k8 * rows + r] = half8_t{v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
       }
     } else {
-      constexpr int NI = kSlabBytes / 32 / (64 * kWaves);  // pieces of 8 columns per thread
-      float4 y[NI][2];
-      float top[NI];
+      constexpr int NI = (slab_bytes<A16, RT>() / 32 + 64 * kWaves - 1) / (64 * kWaves);  // pieces of 8 columns per thread
+      float4 x[NI][2];
       for (int u = threadIdx.x; u < rows; u += 64 * kWaves) top_s[u] = 0u;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int u = threadIdx.x + 64 * kWaves * i, r = u / n8, k8 = u - r * n8;
-        y[i][0] = y[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (u < items) {
           const float* a = static_cast<const float*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8;
-          y[i][0] = *reinterpret_cast<const float4*>(a);
-          y[i][1] = *reinterpret_cast<const float4*>(a + 4);
+          x[i][0] = *reinterpret_cast<const float4*>(a);
+          x[i][1] = *reinterpret_cast<const float4*>(a + 4);
         }
       }
       __syncthreads();
@@ -169,19 +176,20 @@ __global__ __launch_bounds__(64 * kWaves) void linear_i4_kernel(I4Args p) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int u = threadIdx.x + 64 * kWaves * i;
-        const float4 a = y[i][0], b = y[i][1];
-        top[i] = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
-                       fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
-        top[i] = fmaxf(top[i], dpp<kDppXor1>(top[i]));
-        top[i] = fmaxf(top[i], dpp<kDppXor2>(top[i]));
-        if (u < items && (threadIdx.x & 3) == 0) atomicMax(&top_s[u / n8], __builtin_bit_cast(uint32_t, top[i]));
+        const float4 a = x[i][0], b = x[i][1];
+        float top = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
+                          fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
+        top = fmaxf(top, dpp<kDppXor1>(top));
+        top = fmaxf(top, dpp<kDppXor2>(top));
+        if (u < items && (threadIdx.x & 3) == 0) atomicMax(&top_s[u / n8], __builtin_bit_cast(uint32_t, top));
       }
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int u = threadIdx.x + 64 * kWaves * i, r = u / n8, k8 = u - r * n8;
         if (u < items) {
-          const float v[8] = {y[i][0].x, y[i][1].x, y[i][0].y, y[i][1].y, y[i][0].z, y[i][1].z, y[i][0].w, y[i][1].w};
+          const float4 a = x[i][0], b = x[i][1];
+          const float v[8] = {a.x, b.x, a.y, b.y, a.z, b.z, a.w, b.w};
           const int up = i4_up(__builtin_bit_cast(float, top_s[r]));
           half8_t hi, lo;
 #pragma unroll
@@ -315,8 +323,9 @@ __global__ __launch_bounds__(64 * kWaves) void linear_i4_kernel(I4Args p) {
 template <bool A16, int SG, int RT, int NR, int CT, int WK>
 void launch_i4(I4Args p, hipStream_t s) {
   const int rows = p.M < 16 * RT ? p.M : 16 * RT, per = rows * (A16 ? 2 : 4);  // bytes of a column of k
-  p.slab = kSlabBytes / per / kChunk * kChunk;
+  p.slab = slab_bytes<A16, RT>() / per / kChunk * kChunk;
   if (p.slab > p.K) p.slab = p.K;
+  constexpr int kWaves = waves<WK>();
   const size_t red = WK > 1 ? sizeof(float) * kWaves * RT * CT * NR * 64 : 0;
   const size_t lds = std::max<size_t>((size_t)p.slab * per, red);
   const int cols = 16 * CT * (WK == 1 ? kWaves : 1);
@@ -324,19 +333,31 @@ void launch_i4(I4Args p, hipStream_t s) {
   linear_i4_kernel<A16, SG, RT, NR, CT, WK><<<grid, 64 * kWaves, lds, s>>>(p);
 }
 
+// us, fp16 x and 32-column groups unless said otherwise:
+//  - many rows: 32 x 128 blocks from 4096 (fp32 x: 2048) 16 x 16 tiles on, else 16 x 16 blocks whose waves split
+//    K (256 x 4096 x 640 12.4, 32 x 4096 x 640 4.4; as the other 12.7, 5.7);
+//  - up to 16 rows and 65536 columns: a wave per 16 columns (fp32 x or more than 4 rows: 32, since the rows'
+//    operands then cost more) over all of K, each with loads coming for two to four chunks (1 x 262144 x 640
+//    18.2, with 64 columns per wave 23.9, split over K 22.3; 1 x 65536 x 4096 34.5, 42.8, 33.7);
+//  - few columns: K over the sixteen waves of a block (one block per CU or two: 1 x 1536 x 640 fp32 3.6, over
+//    four 4.0; 1 x 8192 x 1536 4.1, 4.7; past that four are better: 4 x 4608 x 1536 fp32 6.6, 7.3).
 template <bool A16, int SG>
 void choose_i4(const I4Args& p, hipStream_t s) {
-  const long long tiles = (p.N + 15) / 16;
-  if (p.M <= 16) {
-    // one wave per 64 columns where that fills the chip, else the chunks of 16 columns over four waves
-    const bool wide = tiles >= 4 * 1024;
-    if (p.M <= 4) wide ? launch_i4<A16, SG, 1, 1, 4, 1>(p, s) : launch_i4<A16, SG, 1, 1, 1, 4>(p, s);
-    else if (p.M <= 8) wide ? launch_i4<A16, SG, 1, 2, 4, 1>(p, s) : launch_i4<A16, SG, 1, 2, 1, 4>(p, s);
-    else wide ? launch_i4<A16, SG, 1, 4, 4, 1>(p, s) : launch_i4<A16, SG, 1, 4, 1, 4>(p, s);
-  } else if (tiles * ((p.M + 31) / 32) < 2048) {
-    launch_i4<A16, SG, 2, 4, 1, 4>(p, s);
+  const long long tiles = (p.N + 15) / 16, units = tiles * ((p.M + 15) / 16);
+  if (p.M > 16 && units >= (A16 ? 4096 : 2048)) {
+    launch_i4<A16, SG, 2, 4, 2, 1>(p, s);
+  } else if (p.M <= 16 && tiles >= 4096) {
+    if (p.M <= 4) launch_i4<A16, SG, 1, 1, A16 ? 1 : 2, 1>(p, s);
+    else if (p.M <= 8) launch_i4<A16, SG, 1, 2, 2, 1>(p, s);
+    else launch_i4<A16, SG, 1, 4, 2, 1>(p, s);
+  } else if (p.K > 4 * kChunk && units <= (A16 ? 512 : 256)) {
+    if (p.M <= 4) launch_i4<A16, SG, 1, 1, 1, 16>(p, s);
+    else if (p.M <= 8) launch_i4<A16, SG, 1, 2, 1, 16>(p, s);
+    else launch_i4<A16, SG, 1, 4, 1, 16>(p, s);
   } else {
-    launch_i4<A16, SG, 4, 4, 2, 1>(p, s);
+    if (p.M <= 4) launch_i4<A16, SG, 1, 1, 1, 4>(p, s);
+    else if (p.M <= 8) launch_i4<A16, SG, 1, 2, 1, 4>(p, s);
+    else launch_i4<A16, SG, 1, 4, 1, 4>(p, s);
   }
 }
 
