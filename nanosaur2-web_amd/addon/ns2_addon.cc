@@ -1004,6 +1004,95 @@ napi_value LinearBf16AddRmsnorm(napi_env env, napi_callback_info info) {
   return check(env, c, ns2_linear_bf16_add_rmsnorm(A, lda, W, bias, x, wa, wo, y, M, N, K, eps));
 }
 
+// quantizeI4(W, codes, scale, N, K, group)
+napi_value QuantizeI4(napi_env env, napi_callback_info info) {
+  ARGS(6);
+  auto W = (const uint16_t*)c.ptr(0);
+  auto codes = (uint8_t*)c.ptr(1);
+  auto scale = (uint16_t*)c.ptr(2);
+  int N = c.i32(3), K = c.i32(4), group = c.i32(5);
+  if (c.failed) return nullptr;
+  return check(env, c, ns2_quantize_i4(W, codes, scale, N, K, group));
+}
+
+// linearI4(A, aFmt, lda, W, scale, bias, add, C, M, N, K, group, ldc, cOff, alpha, act, resid, gate, gOff)
+napi_value LinearI4(napi_env env, napi_callback_info info) {
+  ARGS(19);
+  const void* A = c.ptr(0);
+  int aFmt = c.i32(1), lda = c.i32(2);
+  auto W = (const uint8_t*)c.ptr(3);
+  auto scale = (const uint16_t*)c.ptr(4);
+  auto bias = (const float*)c.ptr(5);
+  auto add = (const float*)c.ptr(6);
+  auto C = (float*)c.ptr(7);
+  int M = c.i32(8), N = c.i32(9), K = c.i32(10), group = c.i32(11), ldc = c.i32(12);
+  long long cOff = c.i64(13);
+  float alpha = c.f32(14);
+  int act = c.i32(15), resid = c.i32(16);
+  auto gate = (const float*)c.ptr(17);
+  long long gOff = c.i64(18);
+  if (c.failed) return nullptr;
+  return check(env, c, ns2_linear_i4(A, aFmt, lda, W, scale, bias, add, C, M, N, K, group, ldc, cOff, alpha, act, resid,
+                                     gate, gOff));
+}
+
+// headNormCache(X, ldx, pos, wQ, wK, cs, sinOff, ropeRows, eps, q, qFmt, ldq, k, v, kGroups, vGroups, batch, L, H, KH, D,
+//               cap, ldkv, kvBatch)
+napi_value HeadNormCache(napi_env env, napi_callback_info info) {
+  ARGS(24);
+  auto X = (const float*)c.ptr(0);
+  int ldx = c.i32(1);
+  auto pos = (const int*)c.ptr(2);
+  auto wq = (const float*)c.ptr(3);
+  auto wk = (const float*)c.ptr(4);
+  auto cs = (const float*)c.ptr(5);
+  long long sinOff = c.i64(6);
+  int ropeRows = c.i32(7);
+  float eps = c.f32(8);
+  void* q = c.ptr(9);
+  int qFmt = c.i32(10), ldq = c.i32(11);
+  void *k = c.ptr(12), *v = c.ptr(13);
+  auto kg = (uint16_t*)c.ptr(14);
+  auto vg = (uint16_t*)c.ptr(15);
+  int batch = c.i32(16), L = c.i32(17), H = c.i32(18), KH = c.i32(19), D = c.i32(20), cap = c.i32(21), ldkv = c.i32(22);
+  long long kvBatch = c.i64(23);
+  if (c.failed) return nullptr;
+  return check(env, c, ns2_head_norm_cache(X, ldx, pos, wq, wk, cs, sinOff, ropeRows, eps, q, qFmt, ldq, k, v, kg, vg, batch, L,
+                                           H, KH, D, cap, ldkv, kvBatch));
+}
+
+// attentionCacheBytes(batch, L, H, KH, D, cap, window, sinks) -> bytes of work memory
+napi_value AttentionCacheBytes(napi_env env, napi_callback_info info) {
+  ARGS(8);
+  int a[8];
+  for (int i = 0; i < 8; ++i) a[i] = c.i32(i);
+  if (c.failed) return nullptr;
+  return number(env, (double)ns2_attention_cache_bytes(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7]));
+}
+
+// attentionCache(q, qFmt, ldq, pos, k, v, kGroups, vGroups, o, ldo, batch, L, H, KH, D, cap, ldkv, kvBatch, window, sinks,
+//                scale, work, workBytes)
+napi_value AttentionCache(napi_env env, napi_callback_info info) {
+  ARGS(23);
+  const void* q = c.ptr(0);
+  int qFmt = c.i32(1), ldq = c.i32(2);
+  auto pos = (const int*)c.ptr(3);
+  const void *k = c.ptr(4), *v = c.ptr(5);
+  auto kg = (const uint16_t*)c.ptr(6);
+  auto vg = (const uint16_t*)c.ptr(7);
+  void* o = c.ptr(8);
+  int ldo = c.i32(9), batch = c.i32(10), L = c.i32(11), H = c.i32(12), KH = c.i32(13), D = c.i32(14), cap = c.i32(15),
+      ldkv = c.i32(16);
+  long long kvBatch = c.i64(17);
+  int window = c.i32(18), sinks = c.i32(19);
+  float scale = c.f32(20);
+  void* work = c.ptr(21);
+  long long bytes = c.i64(22);
+  if (c.failed) return nullptr;
+  return check(env, c, ns2_attention_cache(q, qFmt, ldq, pos, k, v, kg, vg, o, ldo, batch, L, H, KH, D, cap, ldkv, kvBatch,
+                                           window, sinks, scale, work, bytes < 0 ? 0 : (size_t)bytes));
+}
+
 napi_value Module(napi_env env, napi_value exports) {
   struct Fn {
     const char* name;
@@ -1033,6 +1122,8 @@ napi_value Module(napi_env env, napi_value exports) {
       {"partsAddRmsnormTiled", PartsAddRmsnormTiled}, {"linearF16wTiledHeadNormF16kv", LinearF16wTiledHeadNormF16kv},
       {"linearF16wTiledGluDown", LinearF16wTiledGluDown}, {"linearBf16HeadNorm", LinearBf16HeadNorm},
       {"linearBf16HeadNormF16kv", LinearBf16HeadNormF16kv}, {"transpose", Transpose},
+      {"quantizeI4", QuantizeI4}, {"linearI4", LinearI4}, {"headNormCache", HeadNormCache},
+      {"attentionCacheBytes", AttentionCacheBytes}, {"attentionCache", AttentionCache},
   };
   for (const Fn& f : fns) {
     napi_value fn;

@@ -6,12 +6,16 @@
 // heads (causal, through ops.attention's materialized-path kernel); GELU(tanh)-gated MLP. Every
 // 6th layer is global (RoPE theta 1e6), the others local (theta 1e4; their 512-token window
 // never applies at <= 256 tokens).
+//
+// encode() takes a whole prompt and attends causally in every layer, as the reference does. newCache / extend
+// (no counterpart there) take tokens as they come, in any pieces, with the local layers' window, keeping keys and
+// values in a cache of fp16 or 4 bits; load's weightBits: 4 keeps the linears as 4-bit codes.
 
 import * as ops from "./ops.js";
 import { concatLinears } from "./weights.js";
 import { ropeTable } from "./common.js";
 
-export const GEMMA = { layers: 18, hidden: 640, heads: 4, kvHeads: 1, headDim: 256, globalEvery: 6 };
+export const GEMMA = { layers: 18, hidden: 640, heads: 4, kvHeads: 1, headDim: 256, globalEvery: 6, window: 512 };
 const RUN = GEMMA.layers - 1; // layers needed for the penultimate hidden state
 
 // One decoder layer's tensors under the checkpoint's names (app/models/gemma3.js:17-41 reads
@@ -46,8 +50,10 @@ async function loadLayer(gpu, st, i) {
 }
 
 export class Gemma3 {
-  // st: { linear, vector, rows, has } (weights.js SafeTensors or the synthetic source)
-  static async load(gpu, st, onProgress) {
+  // st: { linear, vector, rows, has } (weights.js SafeTensors or the synthetic source). weightBits: 16
+  // (bf16 as stored) or 4 (each linear quantized with an fp16 scale per `group` columns).
+  static async load(gpu, st, onProgress, { weightBits = 16, group = 32 } = {}) {
+    if (weightBits !== 16 && weightBits !== 4) throw new Error(`Gemma3.load: ${weightBits} bits per weight (16 or 4)`);
     const m = new Gemma3(gpu, st);
     m.layers = [];
     for (let i = 0; i < RUN; i++) {
@@ -55,7 +61,10 @@ export class Gemma3 {
       // every linear re-tiled as fp16 (next to its row-major copy): q/k/v and gate/up take the
       // tiled operands the row kernels write, o_proj and down the fused projections of the
       // attention and of the GLU
-      for (const W of [l.qkv, l.o, l.gateUp, l.down]) if (ops.tileablePlain(W)) ops.tileWeight(gpu, W);
+      for (const W of [l.qkv, l.o, l.gateUp, l.down]) {
+        if (weightBits === 4) ops.quantizeI4(gpu, W, group);
+        else if (ops.tileablePlain(W)) ops.tileWeight(gpu, W);
+      }
       m.layers.push(l);
       if (onProgress) onProgress((i + 1) / RUN);
     }
@@ -188,6 +197,102 @@ export class Gemma3 {
     });
     x.release();
     return h; // the final norm of the last layer's output
+  }
+
+  // An empty cache for `batch` sequences of up to `capacity` tokens, keys and values of `bits` 16 or 4. lengths[b] is
+  // the number of tokens that sequence b holds; setting it lower drops what is behind, so that a prompt can be
+  // continued from any of its prefixes. sinks: first tokens that stay visible to the local layers.
+  newCache({ batch = 1, capacity = 1024, bits = 16, sinks = 0 } = {}) {
+    const { kvHeads: KH, headDim: D } = GEMMA;
+    const layers = this.layers.map(() => ops.kvCache(this.gpu, { batch, capacity, KH, D, bits }));
+    return {
+      batch, capacity, bits, sinks, layers, lengths: new Array(batch).fill(0), cs: this.ropeTables(capacity),
+      destroy: () => layers.forEach((c) => c.destroy()),
+    };
+  }
+
+  // The next tokens of a cache's sequences: ids is one array of token ids per sequence (or, for a batch of one, the
+  // array itself), of unequal lengths if need be. Returns the normed hidden states [batch * L, 640], L the longest
+  // array's length; rows b * L + i past a sequence's own tokens hold nothing.
+  async extend(cache, ids) {
+    const lists = cache.batch === 1 && !Array.isArray(ids[0]) ? [ids] : ids;
+    const { pos, L } = this.positions(cache, lists.map((t) => t.length));
+    const padded = [];
+    for (const t of lists) for (let i = 0; i < L; i++) padded.push(i < t.length ? t[i] : t.length ? t[0] : 0);
+    const rows = await this.st.rows("model.embed_tokens.weight", padded);
+    const posT = this.gpu.fromArray(pos, [pos.length]);
+    const y = this.extendEmbedded(cache, this.embed(rows, padded.length), posT, L);
+    posT.release();
+    lists.forEach((t, b) => { cache.lengths[b] += t.length; });
+    return y;
+  }
+
+  // Positions of the next counts[b] tokens of each sequence, -1 for padding up to the longest.
+  positions(cache, counts) {
+    if (counts.length !== cache.batch) throw new Error(`Gemma3: tokens for ${counts.length} of ${cache.batch} sequences`);
+    const L = Math.max(...counts);
+    if (!(L > 0)) throw new Error("Gemma3: no tokens");
+    const pos = new Int32Array(cache.batch * L).fill(-1);
+    counts.forEach((n, b) => {
+      if (cache.lengths[b] + n > cache.capacity) {
+        throw new Error(`Gemma3: sequence ${b} of ${cache.lengths[b]} tokens has no room for ${n} more (capacity ${cache.capacity})`);
+      }
+      for (let i = 0; i < n; i++) pos[b * L + i] = cache.lengths[b] + i;
+    });
+    return { pos, L };
+  }
+
+  // The layer stack on new tokens x [batch * L, 640] (released here) at positions pos (int32 on the device).
+  extendEmbedded(cache, x, pos, L) {
+    const gpu = this.gpu;
+    const { hidden, heads: H } = GEMMA;
+    const [csLocal, csGlobal] = cache.cs;
+    let h = ops.rmsnorm(gpu, x, this.layers[0].inNorm, hidden);
+    this.layers.forEach((l, i) => {
+      const kv = cache.layers[i];
+      const qkv = ops.linear(gpu, h, l.qkv, { name: "te.qkv" });
+      h.release();
+      const q = ops.headNormCache(gpu, qkv, pos, kv, { L, H, wq: l.qn, wk: l.kn, cs: l.global ? csGlobal : csLocal,
+        half: l.o.kind === "i4" });
+      qkv.release();
+      const a = ops.attentionCache(gpu, q, pos, kv, { L, H, window: l.global ? 0 : GEMMA.window, sinks: cache.sinks });
+      q.release();
+      const h2 = ops.linearAddRmsnorm(gpu, a, l.o, x, l.postAttnNorm, l.preMlpNorm);
+      a.release();
+      const g = ops.linearGlu(gpu, h2, l.gateUp, "gelu_tanh");
+      h2.release();
+      h = ops.linearAddRmsnorm(gpu, g, l.down, x, l.postMlpNorm, i + 1 < this.layers.length ? this.layers[i + 1].inNorm : this.norm);
+      g.release();
+    });
+    x.release();
+    return h;
+  }
+
+  // One token of every sequence recorded as a HIP graph. Returns { input [batch, 640], output [batch, 640],
+  // launch(active), destroy() }: write the scaled embeddings into input, launch, then read output. launch takes the
+  // cache's next positions (active[b] false: sequence b has no token this time) and counts them.
+  captureStep(cache) {
+    const gpu = this.gpu;
+    const input = gpu.empty([cache.batch, GEMMA.hidden]);
+    gpu.write(input.buf, new Float32Array(cache.batch * GEMMA.hidden));
+    const pos = gpu.fromArray(new Int32Array(cache.batch).fill(-1), [cache.batch]);
+    const g = gpu.capture(() => this.extendEmbedded(cache, ops.elementwise(gpu, "copy", input), pos, 1));
+    return {
+      input,
+      output: g.result,
+      launch: (active = null) => {
+        const counts = cache.lengths.map((_, b) => (!active || active[b] ? 1 : 0));
+        gpu.write(pos.buf, this.positions(cache, counts).pos);
+        g.launch();
+        counts.forEach((n, b) => { cache.lengths[b] += n; });
+      },
+      destroy: () => {
+        g.destroy();
+        g.result.release();
+        input.release();
+        pos.release();
+      },
+    };
   }
 
   // The local (theta 1e4) and global (1e6) RoPE tables for L tokens, built once per L (they

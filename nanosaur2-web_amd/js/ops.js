@@ -59,6 +59,21 @@ export function tileWeight(gpu, W) {
   return W;
 }
 
+// Turn a bf16 weight into 4-bit codes with an fp16 scale per `group` columns (kind "i4", a quarter of the bytes;
+// its bf16 copies are freed), for linear(). No counterpart in the reference; a LoRA cannot be attached to it.
+export function quantizeI4(gpu, W, group = 32) {
+  if (W.kind !== "bf16" || !W.buf) throw new Error(`${W.name}: only a bf16 weight can be quantized to 4 bits`);
+  if (![32, 64, 128].includes(group) || W.K % group) throw new Error(`${W.name}: K=${W.K} does not take 4-bit groups of ${group}`);
+  if (W.lora && W.lora.length) throw new Error(`${W.name}: quantize before LoRAs are attached, and without them`);
+  const device = (bytes) => new DeviceBuffer(native.malloc(bytes), bytes, false);
+  const codes = device((W.N * W.K) / 2);
+  const scale = device((2 * W.N * W.K) / group);
+  gpu.run("quantize_i4", 0, () => native.quantizeI4(addr(W.buf), addr(codes), addr(scale), W.N, W.K, group));
+  W.buf.destroy();
+  if (W.tbuf) W.tbuf.destroy();
+  return Object.assign(W, { kind: "i4", buf: codes, tbuf: null, scale, group });
+}
+
 // x (- sub) as the tiled fp16 operand of a linear over a re-tiled bf16 weight ([rows, cols],
 // cols % 64 == 0): the DiT's patch-embedder input, and the SPRINT projection's input g - x
 // (app/models/nanosaur2.js:236-243: elementwise sub, then linear) without the fp32 difference.
@@ -141,6 +156,14 @@ export function linear(gpu, x, W, opts = {}) {
   const act = ACT[opts.act || "none"];
   if (act === undefined) throw new Error(`linear: unknown activation ${opts.act}`);
   const resid = opts.resid ? 1 : 0;
+  if (W.kind === "i4") {
+    if (src.tiled) throw new Error(`${W.name}: a 4-bit weight takes row-major rows`);
+    if (W.lora && W.lora.length) throw new Error(`${W.name}: LoRAs on a 4-bit weight are not part of this build`);
+    gpu.run(opts.name || "gemm.i4", 2 * M * W.N * W.K, () =>
+      native.linearI4(addr(src), src.dtype === "f16" ? 1 : 0, W.K, addr(W.buf), addr(W.scale), addr(bias), null, addr(out), M,
+        W.N, W.K, W.group, ldc, cOff, 1, act, resid, addr(opts.gate), gOff));
+    return out;
+  }
   if (W.kind === "i8" && src.tiled && opts.vpack) {
     if (!W.tbuf) throw new Error(`${W.name}: a tiled operand needs the tiled weight (tileWeight)`);
     if (resid) throw new Error("linear: packed values take a plain store (no resid)");
@@ -535,6 +558,57 @@ export function attention(gpu, { q, k, v, Lq, Lk, H, D, ldq, ldk, ldv, qOff = 0,
     native.attention(addr(q), addr(k), addr(v), addr(o), 1, Lq, Lk, H, D, ldq, ldk, ldv, H * D, qOff, kOff, vOff, 0,
       0, 0, 0, 0, 1 / Math.sqrt(D), addr(bias), biasStart, 0, addr(qNorm), addr(kNorm), eps,
       cs ? addr(cs) : null, cs ? cs.sinOff : 0, cs ? ropeRows : 0));
+  return o;
+}
+
+// ---- a key/value cache (additions to the reference ops) -------------------------------------------
+// Buffers for `batch` sequences of up to `capacity` positions: KH key and value heads of D, as fp16 (bits 16) or
+// as 4-bit codes with an fp16 step and offset per 32 values (bits 4). Rows are written by headNormCache before
+// attentionCache sees them; what they hold before that does not matter.
+export function kvCache(gpu, { batch = 1, capacity, KH, D, bits = 16 }) {
+  if (bits !== 16 && bits !== 4) throw new Error(`kvCache: ${bits} bits per value (16 or 4)`);
+  const values = batch * capacity * KH * D;
+  if (!(values > 0)) throw new Error("kvCache: batch, capacity, KH and D must be positive");
+  const device = (bytes) => new DeviceBuffer(native.malloc(bytes), bytes, false);
+  const c = { batch, capacity, KH, D, bits, ldkv: KH * D, kvBatch: capacity * KH * D, kGroups: null, vGroups: null };
+  c.k = device((values * bits) / 8);
+  c.v = device((values * bits) / 8);
+  if (bits === 4) {
+    c.kGroups = device(values / 8);
+    c.vGroups = device(values / 8);
+  }
+  c.destroy = () => {
+    for (const b of [c.k, c.v, c.kGroups, c.vGroups]) if (b) b.destroy();
+  };
+  return c;
+}
+
+// The q|k|v rows x [batch * L, (H + 2 KH) * D] of new tokens at positions pos (int32 [batch * L] on the device; negative:
+// padding): q and k heads normed (wq, wk) and rotated by the table cs at their positions, keys and values into the
+// cache; returns the queries [batch * L, H * D] as fp32, or fp16 (half). Padding rows of the result hold nothing.
+export function headNormCache(gpu, x, pos, cache, { L, H, wq = null, wk = null, cs = null, half = false, eps = 1e-6 }) {
+  const { batch, KH, D, capacity } = cache;
+  const q = gpu.empty([batch * L, H * D], half ? "f16" : "f32");
+  gpu.run("head_norm_cache", 0, () =>
+    native.headNormCache(addr(x), (H + 2 * KH) * D, addr(pos), addr(wq), addr(wk), cs ? addr(cs) : null, cs ? cs.sinOff : 0,
+      cs ? cs.sinOff / (D / 2) : 0, eps, addr(q), half ? 1 : 0, H * D, addr(cache.k), addr(cache.v), addr(cache.kGroups),
+      addr(cache.vGroups), batch, L, H, KH, D, capacity, cache.ldkv, cache.kvBatch));
+  return q;
+}
+
+// Attention of the queries q [batch * L, H * D] (fp32 or fp16; the result has the same type) at positions pos over
+// the cache: position p sees key j <= p if window is 0, j > p - window or j < sinks. Padding rows of the result
+// hold nothing.
+export function attentionCache(gpu, q, pos, cache, { L, H, window = 0, sinks = 0, scale = null }) {
+  const { batch, KH, D, capacity } = cache;
+  const o = gpu.empty([batch * L, H * D], q.dtype);
+  const bytes = native.attentionCacheBytes(batch, L, H, KH, D, capacity, window, sinks);
+  const work = bytes ? gpu.empty([Math.ceil(bytes / 4)]) : null;
+  gpu.run("attn.cache", 0, () =>
+    native.attentionCache(addr(q), q.dtype === "f16" ? 1 : 0, H * D, addr(pos), addr(cache.k), addr(cache.v),
+      addr(cache.kGroups), addr(cache.vGroups), addr(o), H * D, batch, L, H, KH, D, capacity, cache.ldkv, cache.kvBatch, window,
+      sinks, scale === null ? 1 / Math.sqrt(D) : scale, addr(work), bytes));
+  if (work) work.release();
   return o;
 }
 

@@ -3,7 +3,8 @@
 //   node run_gemma.js (--weights FILE.safetensors | --synthetic SEED)
 //                     (--ids FILE.json | --tokens N[,SEED])
 //                     [--out FILE.f32] [--warmup N] [--reps N] [--profile] [--lora FILE[:STRENGTH]]...
-//                     [--graph] [--graph-check N]
+//                     [--graph] [--graph-check N] [--weight-bits 4|16]
+//                     [--cache CAPACITY] [--cache-bits 4|16] [--sinks N] [--chunk N]
 //
 // --ids holds a JSON array of token ids; --tokens draws N seeded ids. --out writes the hidden
 // states [L, 640] as raw fp32. With --reps the encoder is timed on device-resident embeddings
@@ -12,6 +13,9 @@
 // from) its replays instead. --graph-check N replays the graph N times, alternating the
 // embeddings of the ids and of a second seeded id set, with an eager encode between replays,
 // and reports each replay's largest difference from the eager encode of the same ids.
+// --weight-bits 4 quantizes the linears at load. --cache feeds the ids through a key/value cache (of
+// --cache-bits per value) --chunk tokens at a time (all of them by default; single tokens replay a recorded
+// step with --graph) instead of encoding them at once; the local layers then see their window and --sinks first tokens.
 
 import fs from "fs";
 import { GPU } from "./device.js";
@@ -37,6 +41,11 @@ function parseArgs(argv) {
     else if (k === "--profile") a.profile = true;
     else if (k === "--graph") a.graph = true;
     else if (k === "--graph-check") a.graphCheck = Number(next());
+    else if (k === "--weight-bits") a.weightBits = Number(next());
+    else if (k === "--cache") a.cache = Number(next());
+    else if (k === "--cache-bits") a.cacheBits = Number(next());
+    else if (k === "--sinks") a.sinks = Number(next());
+    else if (k === "--chunk") a.chunk = Number(next());
     else if (k === "--lora") {
       const m = /^(.*):(-?[\d.]+)$/.exec(next() || "");
       a.loras.push(m ? { file: m[1], strength: Number(m[2]) } : { file: argv[i], strength: 1 });
@@ -55,6 +64,31 @@ function seededIds([n, seed = 1], vocab) {
   return ids;
 }
 
+// The hidden states [ids.length, 640] of ids fed through a cache, a.chunk tokens at a time.
+async function throughCache(gpu, te, st, ids, a) {
+  const cache = te.newCache({ capacity: a.cache, bits: a.cacheBits || 16, sinks: a.sinks || 0 });
+  const chunk = a.chunk || ids.length;
+  const step = a.graph && chunk === 1 ? te.captureStep(cache) : null;
+  const out = new Float32Array(ids.length * 640);
+  for (let i = 0; i < ids.length; i += chunk) {
+    const part = ids.slice(i, i + chunk);
+    if (step) {
+      const emb = te.embed(await st.rows("model.embed_tokens.weight", part), 1);
+      ops.elementwise(gpu, "copy", emb, null, step.input);
+      emb.release();
+      step.launch();
+      out.set(await gpu.read(step.output), i * 640);
+    } else {
+      const h = await te.extend(cache, part);
+      out.set(await gpu.read(h), i * 640);
+      h.release();
+    }
+  }
+  if (step) step.destroy();
+  cache.destroy();
+  return out;
+}
+
 const median = (xs) => {
   const s = [...xs].sort((p, q) => p - q);
   return s.length ? s[Math.floor(s.length / 2)] : null;
@@ -65,7 +99,7 @@ async function main() {
   const t0 = Date.now();
   const gpu = await GPU.create({ profile: !!a.profile });
   const st = a.weights ? await SafeTensors.open(a.weights) : new SyntheticWeights(a.synthetic || 3, { gemma: true });
-  const te = await Gemma3.load(gpu, st);
+  const te = await Gemma3.load(gpu, st, null, { weightBits: a.weightBits || 16 });
   const loraReports = [];
   if (a.loras.length) {
     const regs = { te: linearRegistry(te) };
@@ -82,6 +116,19 @@ async function main() {
   const rows = await st.rows("model.embed_tokens.weight", ids);
   const report = { tokens: ids.length, load_ms: Date.now() - t0, device: gpu.info, loras: loraReports };
   const L = ids.length;
+  if (a.cache) {
+    const t1 = Date.now();
+    const out = await throughCache(gpu, te, st, ids, a);
+    report.cache = { capacity: a.cache, bits: a.cacheBits || 16, chunk: a.chunk || L, ms: Date.now() - t1 };
+    if (a.out) {
+      fs.writeFileSync(a.out, Buffer.from(out.buffer));
+      report.out = a.out;
+    }
+    if (st.close) st.close();
+    te.unload();
+    process.stdout.write(JSON.stringify(report) + "\n");
+    return;
+  }
   const graph = a.graph || a.graphCheck ? te.captureEncode(L) : null;
   if (graph) report.graph = true;
   // one graph replay on the embeddings emb (device tensor [L, 640])

@@ -102,3 +102,49 @@ def attention_bound(o, vmax, smax, n, D, fp16):
     if fp16:
         return t + vmax * (2.0**-11 + n * 2.0**-25) + o.abs() * 2.0**-11 + 2.0**-24
     return t + vmax * (2.0**-21 + n * 2.0**-36) + o.abs() * 2.0**-23
+
+
+def gemma_hidden(W, ids, window, sinks, cache_bits, device):
+    """The text encoder (17 layers of 640, 4 heads of 256 on one key/value head) with the sliding window of its local
+    layers and keys and values as a cache holds them, in float64. W: name -> tensor."""
+    H, D = 4, 256
+
+    def w(name):
+        return W[name].double().to(device)
+
+    def rms(x, name):
+        return x / (x.square().mean(-1, keepdim=True) + 1e-6).sqrt() * (w(name) + 1)
+
+    def held(x):
+        if cache_bits == 16:
+            return x.half().double()
+        return cache_values(*cache_codes(x.float()))
+
+    x = w("model.embed_tokens.weight")[torch.tensor(ids, device=device)] * math.sqrt(640)
+    L = len(ids)
+    p = torch.arange(L, device=device)
+    for i in range(17):
+        n = f"model.layers.{i}."
+        every = (i + 1) % 6 == 0
+        a = p[:, None].double() / (1e6 if every else 1e4) ** (torch.arange(D // 2, dtype=torch.float64, device=device) * 2 / D)
+
+        def turn(t):
+            u, v = t.chunk(2, -1)
+            c, s = a.cos()[:, None], a.sin()[:, None]
+            return torch.cat([u * c - v * s, v * c + u * s], -1)
+
+        h = rms(x, n + "input_layernorm.weight")
+        q = turn(rms((h @ w(n + "self_attn.q_proj.weight").t()).reshape(L, H, D), n + "self_attn.q_norm.weight"))
+        k = held(turn(rms((h @ w(n + "self_attn.k_proj.weight").t()).reshape(L, 1, D), n + "self_attn.k_norm.weight"))[:, 0])
+        v = held(h @ w(n + "self_attn.v_proj.weight").t())
+        seen = p <= p[:, None]
+        if not every:
+            seen = seen & ((p > p[:, None] - window) | (p < sinks))
+        s = torch.where(seen, (q.transpose(0, 1) @ k.t()) / math.sqrt(D), -math.inf)
+        o = (torch.softmax(s, -1) @ v).transpose(0, 1).reshape(L, H * D)
+        x = x + rms(o @ w(n + "self_attn.o_proj.weight").t(), n + "post_attention_layernorm.weight")
+        h = rms(x, n + "pre_feedforward_layernorm.weight")
+        g = h @ w(n + "mlp.gate_proj.weight").t()
+        g = 0.5 * g * (1 + torch.tanh(math.sqrt(2 / math.pi) * (g + 0.044715 * g**3))) * (h @ w(n + "mlp.up_proj.weight").t())
+        x = x + rms(g @ w(n + "mlp.down_proj.weight").t(), n + "post_feedforward_layernorm.weight")
+    return rms(x, "model.norm.weight")
