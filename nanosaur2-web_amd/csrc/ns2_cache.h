@@ -174,17 +174,19 @@ __device__ __forceinline__ int qdim(int t, int grp) {
   return I4 ? grp * (D / 4) + 8 * t : 32 * t + 8 * grp;
 }
 
-// Column m's query (zeros for padding). fp32 queries are scaled by a power of two to below 2^14 and taken as two
-// halves that keep 22 bits.
+// Column m's query (zeros for padding), negated for a negative scale. fp32 queries are scaled by a power of two to
+// below 2^14 and taken as two halves that keep 22 bits.
 template <int D, bool I4, bool F32>
 struct Query {
   static constexpr int QT = D / 32;
   float4 x[F32 ? QT : 1][2];
   half8_t h[F32 ? 1 : QT];
+  float sign;
 
   __device__ __forceinline__ void load(const AttnArgs& a, int b, int g, int m, bool live, int grp) {
     const int G = a.H / a.KH, i = live ? m / G : 0, hd = live ? m - i * G : 0;
     const long long e = ((long long)b * a.L + i) * a.ldq + (long long)(g * G + hd) * D;
+    sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       const int d = qdim<D, I4>(t, grp);
@@ -209,18 +211,20 @@ struct Query {
     top = column_max(top);
     return top > 0.f && top < INFINITY ? min(14 - __builtin_amdgcn_frexp_expf(top), 120) : 0;
   }
+  // What takes a score to a base-2 logarithm: above 0, so that -inf stays -inf for a scale of 0.
+  __device__ __forceinline__ static float mult(const AttnArgs& a, int up) { return fmaxf(ldexpf(fabsf(a.scale), -up), 1e-37f); }
   // The B operand of step t; PERM: in the order of dequant8.
   template <bool PERM>
   __device__ __forceinline__ void operand(int t, int up, half8_t& hi, half8_t& lo) const {
     constexpr int order[8] = {0, PERM ? 4 : 1, PERM ? 1 : 2, PERM ? 5 : 3, PERM ? 2 : 4, PERM ? 6 : 5, PERM ? 3 : 6, 7};
     if constexpr (!F32) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) hi[e] = h[t][order[e]];
+      for (int e = 0; e < 8; ++e) hi[e] = h[t][order[e]] * (half_t)sign;
     } else {
       const float y[8] = {x[t][0].x, x[t][0].y, x[t][0].z, x[t][0].w, x[t][1].x, x[t][1].y, x[t][1].z, x[t][1].w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float z = ldexpf(y[order[e]], up);
+        const float z = ldexpf(sign * y[order[e]], up);
         hi[e] = (half_t)z;
         lo[e] = (half_t)(z - (float)hi[e]);
       }
@@ -236,14 +240,14 @@ struct Query {
 // smallest (a weight's rounding is off by 2^-25 at least, 2^-31 of the weight of the reference).
 constexpr float kSlack = 8.f, kLift = 6.f;
 
-// Scores s[N] (base-2 logarithms, -inf where masked) of the lane's column -> weights in place; returns
-// whether the lane's column moved its reference, with the factor for what was summed before.
+// Scores s[N] (-inf where masked; times mult > 0 they are base-2 logarithms) of the lane's column -> weights in
+// place; returns whether the lane's column moved its reference, with the factor for what was summed before.
 template <int N>
-__device__ __forceinline__ bool soften(float (&s)[N], float& m, float& l, float& corr) {
+__device__ __forceinline__ bool soften(float (&s)[N], float mult, float& m, float& l, float& corr) {
   float top = s[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) top = fmaxf(top, s[i]);
-  top = column_max(top);
+  top = column_max(top) * mult;
   const bool moves = top > m + kSlack;
   corr = moves && m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : moves ? 0.f : 1.f;
   m = moves ? top : m;
@@ -251,7 +255,7 @@ __device__ __forceinline__ bool soften(float (&s)[N], float& m, float& l, float&
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], mult, -ref));
     sum += s[i];
   }
   l = l * corr + sum;

@@ -7,6 +7,7 @@
 // to a byte (the even value in the low four bits) and, per 32 values, an fp16 step s and offset o;
 // it stands for the fp16 values half(o + c*s).
 #include <algorithm>
+#include <cmath>
 
 #include "ns2_cache.h"
 
@@ -306,6 +307,7 @@ int ns2_attention_cache(const void* q, int q_fmt, int ldq, const int* pos, const
   NS2_REQUIRE(o && aligned(o, 16) && ldo >= H * D && ldo % (q_fmt ? 8 : 4) == 0,
               "%s: o must hold 16-byte aligned rows of H * D values (ldo=%d)", fn, ldo);
   NS2_REQUIRE(window >= 0 && sinks >= 0, "%s: negative window or sinks", fn);
+  NS2_REQUIRE(std::isfinite(scale), "%s: the scale is not a finite number", fn);
   const size_t need = ns2_attention_cache_bytes(batch, L, H, KH, D, cap, window, sinks);
   NS2_REQUIRE(work_bytes >= need && (!need || (work && aligned(work, 16))),
               "%s: the call needs %zu bytes of 16-byte aligned work memory (ns2_attention_cache_bytes), got %zu", fn, need, work_bytes);

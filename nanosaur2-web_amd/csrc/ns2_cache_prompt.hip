@@ -202,7 +202,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
     Query<D, false, F32> query;
     query.load(a, b, g, mc, p[c] >= 0, grp);
     const int up = query.up();
-    mult[c] = ldexpf(a.scale, -up);
+    mult[c] = query.mult(a, up);
 #pragma unroll
     for (int i = 0; i < QT; ++i) query.template operand<I4>(i, up, qh[c][i], ql[c][F32 ? i : 0]);
     m[c] = -INFINITY;
@@ -257,15 +257,17 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
     for (int c = 0; c < CT; ++c) {
       float w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = s[c][i >> 2][i & 3] * mult[c];
+      for (int i = 0; i < 8; ++i) w[i] = s[c][i >> 2][i & 3];
       if (!tile.whole) {
         const Sight sight = sight_of(a, keys, t, p[c]);
+        int key = tile.key0 + 32 * half + 4 * grp;
+        asm volatile("" : "+v"(key));  // (keeps the comparisons below out of whole tiles' way)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (!sight(tile.key0 + 32 * half + 16 * (i >> 2) + 4 * grp + (i & 3))) w[i] = -INFINITY;
+          if (!sight(key + 16 * (i >> 2) + (i & 3))) w[i] = -INFINITY;
       }
       float corr;
-      const bool moves = soften(w, m[c], l[c], corr);
+      const bool moves = soften(w, mult[c], m[c], l[c], corr);
       if (__builtin_amdgcn_ballot_w64(moves)) {
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[c][i] *= corr;

@@ -230,7 +230,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) 
   }
   __builtin_amdgcn_sched_barrier(0);
   const int up = query.up();
-  const float mult = ldexpf(a.scale, -up);
+  const float mult = query.mult(a, up);
 #pragma unroll
   for (int i = 0; i < QT; ++i)
     if (i % kWaves == wave) {
@@ -265,18 +265,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) 
         }
       }
 #pragma unroll
-      for (int i = 0; i < NK; ++i) s[i] = sc[i >> 2][i & 3] * mult;
+      for (int i = 0; i < NK; ++i) s[i] = sc[i >> 2][i & 3];
     }
     const Tile next = tile_of<kTile>(a, keys, tn < t_end ? tn : t);
     const Sight sight = sight_of(a, keys, t, p);
     if (tn < t_end) kx.load(a, base, next, col, grp);
     if (!tile.whole) {
+      int key = tile.key0 + 4 * grp;
+      asm volatile("" : "+v"(key));  // (keeps the comparisons below out of whole tiles' way)
 #pragma unroll
       for (int i = 0; i < NK; ++i)
-        if (!sight(tile.key0 + key_of(grp, i))) s[i] = -INFINITY;
+        if (!sight(key + (i < 4 ? i : 12 + i))) s[i] = -INFINITY;
     }
     float corr;
-    const bool moves = soften(s, m, l, corr);
+    const bool moves = soften(s, mult, m, l, corr);
     if (__builtin_amdgcn_ballot_w64(moves)) {
 #pragma unroll
       for (int i = 0; i < DT; ++i) o[i] *= corr;

@@ -524,3 +524,23 @@ def test_work_memory_is_checked(ns2lib):
     ns2lib.attention_cache(q, pos, kv, kv, o, ldq=1024, ldo=1024, **a)
     a.update(batch=1, L=0)
     ns2lib.attention_cache(q, pos, kv, kv, o, ldq=1024, ldo=1024, **a)
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("scale", [0.0, -0.07])
+def test_scales_that_are_not_positive(ns2lib, scale, fp16):
+    """A scale of 0 weighs all visible keys alike, a negative one prefers the opposite keys; one that is no number is
+    refused."""
+    import ns2
+
+    rnd = gen(41)
+    cache = Cache(rnd, 2, 200, 2, 96, False)
+    for L in (1, 70):
+        pos = positions([(120, L), (3, L)], L)
+        q = rnd(2, L, 8, 96)
+        got = attend(ns2lib, cache, q, pos, 50, 3, fp16, scale=scale)
+        qd = (q.half() if fp16 else q.float()).double()
+        ref, vmax, smax, n = R.attention(qd, pos, cache.value["k"], cache.value["v"], 50, 3, scale)
+        assert ((got.double() - ref).abs() <= R.attention_bound(ref, vmax, smax.abs(), n, 96, fp16)).all()
+        with pytest.raises(ns2.NS2Error, match="scale"):
+            attend(ns2lib, cache, q, pos, 50, 3, fp16, scale=math.nan)
