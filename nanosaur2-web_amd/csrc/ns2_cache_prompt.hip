@@ -144,9 +144,11 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
   const int half = wave >> 2, tid = threadIdx.x & (kHalf - 1);  // waves 0-3: first half of a tile, bring K
   const int col = lane & 15, grp = lane >> 4;
   const int G = a.H / a.KH, R = a.L * G;
-  // Blocks go to the eight dies in turn. Where all of a sequence is visible, its columns with the most keys go
-  // first; in a window, where neighbours share keys, each die takes a run of columns.
-  int by = gridDim.y - 1 - blockIdx.y, bx = blockIdx.x;
+  // Blocks go to the eight dies in turn, the columns with the most keys first. A die would see few of the
+  // heads then (fewer keys for its cache) but also few of the sequences, which may differ in length: every four
+  // column blocks the sequences move on by one (2 and 3 thousand tokens over a 4-bit cache: 316 us without, 262
+  // with; two equal sequences 365, 374). In a window, where neighbours share keys, each die takes a run of columns.
+  int by = gridDim.y - 1 - blockIdx.y, bx = (blockIdx.x + blockIdx.y / 4 * (a.KH * a.splits)) % gridDim.x;
   if (a.window) {
     const int n = gridDim.x * gridDim.y, id = blockIdx.x + gridDim.x * blockIdx.y, even = n / 8, odd = n - 8 * even;
     const int die = id & 7, at = die * even + min(die, odd) + (id >> 3);
