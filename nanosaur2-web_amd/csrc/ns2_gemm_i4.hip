@@ -339,8 +339,11 @@ void launch_i4(I4Args p, hipStream_t s) {
 //  - up to 16 rows and 65536 columns: a wave per 16 columns (fp32 x or more than 4 rows: 32, since the rows'
 //    operands then cost more) over all of K, each with loads coming for two to four chunks (1 x 262144 x 640
 //    18.2, with 64 columns per wave 23.9, split over K 22.3; 1 x 65536 x 4096 34.5, 42.8, 33.7);
-//  - few columns: K over the sixteen waves of a block (one block per CU or two: 1 x 1536 x 640 fp32 3.6, over
-//    four 4.0; 1 x 8192 x 1536 4.1, 4.7; past that four are better: 4 x 4608 x 1536 fp32 6.6, 7.3).
+//  - few columns: K over the sixteen waves of a block where that is one block per CU or two (1 x 1536 x 640 fp32
+//    3.6, over four 4.0; 1 x 8192 x 1536 4.1, 4.7), 32 columns each where fp32 rows would be read by 512 blocks
+//    (5 x 8192 x 1536 fp32 5.6, with 16 columns 7.5, over four waves 6.7);
+//  - else over four waves, 32 columns each (8 x 16384 x 4096 fp32 26.4, with 16 columns 38.1; up to four fp16
+//    rows cost too little for that: 2 x 20000 x 640 4.3, 4.0).
 template <bool A16, int SG>
 void choose_i4(const I4Args& p, hipStream_t s) {
   const long long tiles = (p.N + 15) / 16, units = tiles * ((p.M + 15) / 16);
@@ -354,10 +357,16 @@ void choose_i4(const I4Args& p, hipStream_t s) {
     if (p.M <= 4) launch_i4<A16, SG, 1, 1, 1, 16>(p, s);
     else if (p.M <= 8) launch_i4<A16, SG, 1, 2, 1, 16>(p, s);
     else launch_i4<A16, SG, 1, 4, 1, 16>(p, s);
+  } else if (!A16 && p.K > 4 * kChunk && units <= 512) {
+    if constexpr (!A16) {
+      if (p.M <= 4) launch_i4<A16, SG, 1, 1, 2, 16>(p, s);
+      else if (p.M <= 8) launch_i4<A16, SG, 1, 2, 2, 16>(p, s);
+      else launch_i4<A16, SG, 1, 4, 2, 16>(p, s);
+    }
   } else {
-    if (p.M <= 4) launch_i4<A16, SG, 1, 1, 1, 4>(p, s);
-    else if (p.M <= 8) launch_i4<A16, SG, 1, 2, 1, 4>(p, s);
-    else launch_i4<A16, SG, 1, 4, 1, 4>(p, s);
+    if (p.M <= 4) launch_i4<A16, SG, 1, 1, A16 ? 1 : 2, 4>(p, s);
+    else if (p.M <= 8) launch_i4<A16, SG, 1, 2, 2, 4>(p, s);
+    else launch_i4<A16, SG, 1, 4, 2, 4>(p, s);
   }
 }
 
