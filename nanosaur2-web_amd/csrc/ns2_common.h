@@ -138,18 +138,32 @@ __device__ __forceinline__ float h4_bits23(float v) {
   return t + dpp<kDppHalfMirror>(dpp<kDppRowMirror>(e));
 }
 
-// v_permlane16_swap / v_permlane32_swap (gfx950) as inline assembly: both registers are
-// outputs, and the compiler's builtin returns the first operand's new value for both. The
-// s_nop gives the two wait states these instructions need after a VALU write of an operand.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
+// v_permlane16_swap / v_permlane32_swap (gfx950). Not as inline assembly: the compiler gives a matrix
+// product's unused result registers away while the product still runs and waits before an instruction that
+// writes them, but not before an assembly statement, whose result the product then overwrites. (The results go
+// through variables: a bit cast of the builtin's second result itself would read the first.)
+__device__ __forceinline__ void permlane16_swap(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+__device__ __forceinline__ void permlane32_swap(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
 __device__ __forceinline__ void permlane16_swap(float& a, float& b) {
-  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+  permlane16_swap(x, y);
+  a = __builtin_bit_cast(float, x);
+  b = __builtin_bit_cast(float, y);
 }
 __device__ __forceinline__ void permlane32_swap(float& a, float& b) {
-  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+  permlane32_swap(x, y);
+  a = __builtin_bit_cast(float, x);
+  b = __builtin_bit_cast(float, y);
 }
-#pragma clang diagnostic pop
 
 // Sum over the 64 lanes of a wave, every lane gets it, without LDS traffic: quad sums by DPP
 // (lane ^ 1, ^ 2), then the other quad of the 8-lane half row (half-row mirror), the other
@@ -288,11 +302,11 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
 // The four nibbles n of each 16-bit half of x as half2 pairs, (n0, n0') first, each plus `even` + 1024 (nibbles
 // 0 and 2) or `odd` + 64 (1 and 3): 0x6400 | n is the half 1024 + n, 0x6400 | 16 n the half 1024 + 16 n, and both
 // steps are exact for sums that are small integers. The mask is one instruction with the or (v_and_or_b32
-// takes one scalar operand: the mask; the compiler would split it in two with literals).
+// takes one scalar operand: the mask; the compiler would split it in two with literals, which it does not see).
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
-  uint32_t r;
-  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "s"(mask), "v"(bits));
-  return r;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(bits));
+  return (x & mask) | bits;
 }
 __device__ __forceinline__ void nibbles4(uint32_t x, half2_t even, half2_t odd, uint32_t r[4]) {
   const half2_t sixteenth = {0.0625f, 0.0625f};

@@ -57,16 +57,11 @@ __device__ __forceinline__ void store_i4(const I4Args& p, int m, int n, float ac
 // scales.
 
 // Four registers of the four 16-lane rows transposed: register j of row g becomes register g of row j.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) { asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
-__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) { asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
-#pragma clang diagnostic pop
 __device__ __forceinline__ void transpose_rows(uint32_t w[4]) {
-  swap32(w[0], w[2]);
-  swap32(w[1], w[3]);
-  swap16(w[0], w[1]);
-  swap16(w[2], w[3]);
+  permlane32_swap(w[0], w[2]);
+  permlane32_swap(w[1], w[3]);
+  permlane16_swap(w[0], w[1]);
+  permlane16_swap(w[2], w[3]);
 }
 
 // code - 8 of a word's eight codes
@@ -227,10 +222,10 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
             t[c][3] = w[sl][c].w;
             const float f = (float)sc[sl][c];
             uint32_t a = __builtin_bit_cast(uint32_t, f), b = a;
-            swap32(a, b);  // the scales of steps 0, 1 | 2, 3
+            permlane32_swap(a, b);  // the scales of steps 0, 1 | 2, 3
             uint32_t a1 = a, b1 = b;
-            swap16(a, a1);
-            swap16(b, b1);
+            permlane16_swap(a, a1);
+            permlane16_swap(b, b1);
             s[c][0] = __builtin_bit_cast(float, a);
             s[c][1] = __builtin_bit_cast(float, a1);
             s[c][2] = __builtin_bit_cast(float, b);
@@ -413,7 +408,7 @@ int ns2_quantize_i4(const uint16_t* W, uint8_t* codes, uint16_t* scale, int N, i
   NS2_REQUIRE(N > 0 && K > 0 && K % group == 0, "ns2_quantize_i4: N=%d, K=%d must be positive, K a multiple of the group %d", N, K,
               group);
   const long long groups = (long long)N * (K / group);
-  NS2_REQUIRE((groups + 255) / 256 <= INT32_MAX, "ns2_quantize_i4: %lld groups are too many for one launch", groups);
+  NS2_REQUIRE(groups <= UINT32_MAX - 255LL, "ns2_quantize_i4: %lld groups are too many for one launch", groups);
   ns2::ProfScope prof_("quantize_i4");
   quantize_i4_kernel<<<(unsigned)((groups + 255) / 256), 256, 0, ns2::stream()>>>(W, codes, reinterpret_cast<half_t*>(scale),
                                                                                  groups, group);
@@ -437,7 +432,7 @@ int ns2_linear_i4(const void* A, int a_fmt, int lda, const uint8_t* W, const uin
   NS2_REQUIRE(act >= NS2_ACT_NONE && act <= NS2_ACT_GELU_TANH, "%s: unknown activation %d", fn, act);
   NS2_REQUIRE(aligned(A, 16) && lda % (a_fmt ? 8 : 4) == 0 && aligned(W, 16) && aligned(scale, 2),
               "%s: the rows of A and W must be 16-byte aligned (lda a multiple of %d)", fn, a_fmt ? 8 : 4);
-  NS2_REQUIRE(M <= 16LL * 65535, "%s: M=%d is too many rows for one launch", fn, M);
+  NS2_REQUIRE(M <= 16LL * 65535 && N <= 1 << 29, "%s: M=%d, N=%d are too many for one launch", fn, M, N);
   I4Args p{A,  W,   reinterpret_cast<const half_t*>(scale), bias, add, C, gate, cOff, gOff, lda, ldc, M, N, K, group, alpha,
            act, resid};
   ns2::ProfScope prof_("linear_i4");

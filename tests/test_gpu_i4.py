@@ -150,6 +150,30 @@ def test_many_columns(ns2lib):
         check(run(ns2lib, rnd(M, 640), codes, scale, 64, fp16=True, K=640), f"{M}x50001")
 
 
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(130, 8200, 384), (33, 30011, 256), (17, 65537, 128), (48, 14003, 1408),  # many rows and columns
+                                   (1, 65553, 640), (4, 65600, 1152), (6, 65539, 256), (12, 65553, 384), (16, 66000, 128),  # a table
+                                   (1, 8181, 640), (7, 8177, 1408), (16, 5003, 640), (40, 2050, 896),  # K over sixteen waves
+                                   (1, 20003, 1664), (8, 20003, 640), (16, 10007, 512), (90, 3001, 640)])  # over four
+def test_blocks_of_every_size(ns2lib, M, N, K, group, fp16):
+    g, rnd = gen(M + N)
+    codes, scale = weight(g, N, K, group)
+    check(run(ns2lib, rnd(M, K), codes, scale, group, fp16=fp16, K=K, bias=rnd(N), act="silu", pad=1), f"{M}x{N}x{K} group {group} fp16={fp16}")
+
+
+@pytest.mark.parametrize("M,N,K", [(9, 300, 1536), (5, 66000, 256), (40, 9000, 512)])
+def test_rows_of_any_magnitude(ns2lib, M, N, K):
+    """fp32 rows far below and beyond fp16's range, some of them changing their magnitude along the row, a row of zeros."""
+    g, rnd = gen(N)
+    codes, scale = weight(g, N, K, 64)
+    x = rnd(M, K)
+    for r, f in ((0, 1e-30), (1, 1e-12), (2, 1e6), (3, 1e30), (4, 0.0)):
+        x[r] *= f
+    x[1, K // 2:] *= 1e4
+    check(run(ns2lib, x, codes, scale, 64, fp16=False, K=K), f"{M}x{N}x{K}")
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_quantizer(ns2lib, group):
     """Codes and scales equal the definition; zeros, one strong value, tiny groups, values on a border."""
@@ -181,7 +205,7 @@ def test_quantizer(ns2lib, group):
 
 
 @pytest.mark.parametrize("change", [dict(group=16), dict(group=48), dict(K=80), dict(K=0), dict(N=0), dict(N=-1), dict(M=-1), dict(a_fmt=2),
-                                    dict(lda=120), dict(lda=130), dict(ldc=30), dict(cOff=-1), dict(gOff=-1), dict(act=3), dict(A=4),
+                                    dict(lda=120), dict(lda=130), dict(ldc=30), dict(cOff=-1), dict(gOff=-1), dict(act=3), dict(N=(1 << 29) + 1, ldc=1 << 30), dict(M=1 << 20), dict(A=4),
                                     dict(W=8), dict(scale=1), dict(A=None), dict(W=None), dict(scale=None), dict(C=None)])
 def test_refusals(ns2lib, change):
     import ns2
