@@ -188,9 +188,10 @@ int ns2_tile_bf16_weight(const uint16_t* W, uint16_t* Wt, int N, int K);
  * group 32, 64 or 128, K % group == 0. The same epilogue as above. a_fmt = 0: A is fp32, = 1: fp16
  * ([M, lda]). The products are exact (an fp32 activation takes part as a sum of fp16 parts that
  * keeps 22 of its bits) and summed in fp32, so the result is that of an fp32 linear on the weights
- * that the codes stand for; an fp32 activation beyond fp16's range (65504) is not taken. Made for the
- * few rows of single tokens and conditioning vectors; any M runs. Rows of A and W 16-byte aligned.
- * No counterpart in the reference. */
+ * that the codes stand for. (The parts are taken after scaling by a power of two per row: a value
+ * below 2^-16 of its row's largest keeps fewer bits, none below 2^-39 of it.) Made for the few rows
+ * of single tokens and conditioning vectors; any M runs. Rows of A and W 16-byte aligned, M at most
+ * 2^20 - 16, N 2^29. No counterpart in the reference. */
 int ns2_linear_i4(const void* A, int a_fmt, int lda, const uint8_t* W, const uint16_t* scale,
                   const float* bias, const float* add, float* C, int M, int N, int K, int group,
                   int ldc, long long cOff, float alpha, int act, int resid, const float* gate,
@@ -277,7 +278,7 @@ int ns2_attention_rows_f16kv_oproj(const float* q, const uint16_t* k, const uint
  * v_groups an fp16 step s and offset o (2 halfs) per 32 values; such a cache stands for the fp16
  * values half(o + code * s). D is 64, 96, 128 or 256. q_fmt is the type of q (and o): 0 fp32, 1 fp16.
  * Rows of X, q, o and the cache are 16-byte aligned (ldkv, kvBatch multiples of 8 for fp16, of 32
- * for 4 bits); ldkv is at most 2^24.
+ * for 4 bits); ldkv is at most 2^24, cap 2^30, batch * KH 2^22.
  *
  * ns2_head_norm_cache: X fp32 [batch*L, ldx] holds H query heads, KH key heads and KH value heads
  * (a q|k|v product). Query and key heads are RMS-normed with w_q / w_k [D] (NULL: not normed) and,
@@ -292,7 +293,8 @@ int ns2_attention_rows_f16kv_oproj(const float* q, const uint16_t* k, const uint
  *   j < sinks or j > p - window (window = 0: all j <= p).
  * What the cache holds at other positions, infinities and NaN too, does not matter. kvBatch = 0 lets
  * all sequences read one cache. fp16 q: the softmax weights are rounded to fp16 for the second
- * product; fp32 q: queries and weights take part as sums of fp16 parts that keep 22 of their bits.
+ * product; fp32 q: queries and weights take part as sums of fp16 parts that keep 22 of their bits
+ * (of a query value below 2^-16 of its head's largest, fewer). o must not overlap q.
  * Sums and softmax statistics are fp32; the same call gives the same bits again. work:
  * ns2_attention_cache_bytes bytes of device memory that the call may write (NULL where that is 0);
  * calls that may overlap take one each. */

@@ -30,7 +30,7 @@ struct AttnArgs {
   float2* part_s;  // and their (maximum, sum of weights)
   long long kvBatch;
   int ldq, ldo, ldkv, L, H, KH, cap, window, sinks, q_fmt, batch, splits;
-  float scale;  // times log2(e)
+  float scale;  // the caller's times log2(e)
 };
 
 struct Plan {

@@ -84,12 +84,13 @@ __global__ __launch_bounds__(256) void cache_write_kernel(WriteArgs a) {
     float x[4] = {xs[i].x, xs[i].y, xs[i].z, xs[i].w};
     const bool is_v = h[i] >= (unsigned)(a.H + a.KH), is_q = h[i] < (unsigned)a.H;
     const float* w = is_q ? a.w_q : is_v ? nullptr : a.w_k;
-    const float ss = unit8_sum((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]));
+    // (multiply-adds are written out, so that a token's bits do not depend on U)
+    const float ss = unit8_sum(fmaf(x[0], x[0], x[1] * x[1]) + fmaf(x[2], x[2], x[3] * x[3]));
     float sum = 0.f;
 #pragma unroll
     for (int n = 0; n < D / 32; ++n) sum += __shfl(ss, (base + 8 * n) & 63);
     if (w) {
-      const float r = rsqrtf(sum / (float)D + a.eps);
+      const float r = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
       const float4 w4 = *reinterpret_cast<const float4*>(w + 4 * t);
       x[0] = x[0] * r * w4.x;
       x[1] = x[1] * r * w4.y;
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(WriteArgs a) {
       for (int e = 0; e < 4; ++e) o[e] = __shfl(x[e], partner);
       if (a.cs && !is_v && p[i] >= 0 && p[i] < a.rope_rows) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = x[e] * c[e] + (low ? -o[e] : o[e]) * s[e];
+        for (int e = 0; e < 4; ++e) x[e] = fmaf(x[e], c[e], (low ? -o[e] : o[e]) * s[e]);
       }
     }
     const bool held = lives[i] && p[i] >= 0 && p[i] < a.cap;
@@ -220,13 +221,15 @@ constexpr int kRowsColumns = 64;  // columns of a K/V head up to which its keys 
 constexpr long long kCUs = 256;
 
 Plan plan_of(int batch, int L, int H, int KH, int cap, int window, int sinks) {
-  const long long R = (long long)L * (H / KH), heads = (long long)batch * KH;
+  const long long R = (long long)L * (H / KH);
   // keys that a block may have to read
   const long long keys = window ? std::min<long long>(cap, (long long)window + sinks + L) : cap;
   Plan p;
   p.prompt = R > kRowsColumns;
-  const long long blocks = heads * (p.prompt ? (R + 63) / 64 : (R + 15) / 16);
-  const long long want = p.prompt ? kCUs / blocks : 2 * kCUs / blocks;
+  // enough blocks for the CUs: one each, of few columns two
+  const long long full = p.prompt ? kCUs : 2 * kCUs;
+  const long long heads = std::min((long long)batch * KH, full), tiles = std::min(p.prompt ? (R + 63) / 64 : (R + 15) / 16, full);
+  const long long want = full / (heads * tiles);
   // at least 64 keys per split
   const long long most = std::min<long long>(kMaxSplits, std::max<long long>(1, keys / 64));
   p.splits = (int)std::max<long long>(1, std::min(want, most));
@@ -240,8 +243,10 @@ int check_cache(const char* fn, const void* q, const int* pos, const void* k, co
   NS2_REQUIRE(D == 64 || D == 96 || D == 128 || D == 256, "%s: head dim %d is not 64, 96, 128 or 256", fn, D);
   NS2_REQUIRE(H > 0 && KH > 0 && H % KH == 0 && (long long)H * D <= INT32_MAX, "%s: H=%d is not a positive multiple of KH=%d", fn, H,
               KH);
-  NS2_REQUIRE(cap > 0 && ldq >= H * D && ldkv >= (long long)KH * D && ldkv <= 1 << 24 && kvBatch >= 0,
+  NS2_REQUIRE(cap > 0 && cap <= 1 << 30 && ldq >= H * D && ldkv >= (long long)KH * D && ldkv <= 1 << 24 && kvBatch >= 0,
               "%s: bad sizes or strides (cap=%d, ldq=%d, ldkv=%d)", fn, cap, ldq, ldkv);
+  NS2_REQUIRE((long long)batch * L <= INT32_MAX && (long long)batch * L * (H / KH) <= INT32_MAX - 256 && (long long)batch * KH <= 1 << 22,
+              "%s: batch=%d, L=%d, H=%d are too many for one launch", fn, batch, L, H);
   NS2_REQUIRE(!kg == !vg, "%s: a 4-bit cache needs the groups of both k and v", fn);
   NS2_REQUIRE(q_fmt == 0 || q_fmt == 1, "%s: q_fmt %d is not 0 (fp32) or 1 (fp16)", fn, q_fmt);
   NS2_REQUIRE(aligned(q, 16) && ldq % (q_fmt ? 8 : 4) == 0 && aligned(pos, 4), "%s: the rows of q must be 16-byte aligned", fn);
@@ -270,7 +275,7 @@ int ns2_head_norm_cache(const float* X, int ldx, const int* pos, const float* w_
     NS2_REQUIRE(aligned(cs, 16) && sin_off % 4 == 0 && rope_rows >= 0 && sin_off >= 0, "%s: the rotation table must be 16-byte aligned",
                 fn);
   NS2_REQUIRE(batch == 1 || kvBatch >= (cap - 1LL) * ldkv + KH * D, "%s: the sequences' caches overlap (kvBatch)", fn);
-  const long long units = (long long)batch * L * (H + 2LL * KH);
+  const long long units = (long long)batch * L * (H + 2LL * KH);  // (below 2^55: batch * L and H + 2 KH are)
   NS2_REQUIRE(units <= INT32_MAX, "%s: %lld heads are too many for one launch", fn, units);
   WriteArgs a{X,  pos, w_q, w_k,  cs,   q, k, v, reinterpret_cast<half2_t*>(k_groups), reinterpret_cast<half2_t*>(v_groups), sin_off, kvBatch,
               (unsigned)units, ldx, ldq, ldkv, L, H, KH, cap, rope_rows, q_fmt, eps};
@@ -307,12 +312,10 @@ int ns2_attention_cache(const void* q, int q_fmt, int ldq, const int* pos, const
   NS2_REQUIRE(o && aligned(o, 16) && ldo >= H * D && ldo % (q_fmt ? 8 : 4) == 0,
               "%s: o must hold 16-byte aligned rows of H * D values (ldo=%d)", fn, ldo);
   NS2_REQUIRE(window >= 0 && sinks >= 0, "%s: negative window or sinks", fn);
-  NS2_REQUIRE(std::isfinite(scale), "%s: the scale is not a finite number", fn);
+  NS2_REQUIRE(std::isfinite(scale * kLog2e), "%s: the scale is not a finite number", fn);
   const size_t need = ns2_attention_cache_bytes(batch, L, H, KH, D, cap, window, sinks);
   NS2_REQUIRE(work_bytes >= need && (!need || (work && aligned(work, 16))),
               "%s: the call needs %zu bytes of 16-byte aligned work memory (ns2_attention_cache_bytes), got %zu", fn, need, work_bytes);
-  NS2_REQUIRE((long long)L * (H / KH) <= INT32_MAX - 256 && (long long)batch * KH * 64 <= INT32_MAX,
-              "%s: batch=%d, L=%d, H=%d are too many for one launch", fn, batch, L, H);
   const Plan plan = plan_of(batch, L, H, KH, cap, window, sinks);
   NS2_REQUIRE((long long)L * (H / KH) <= 64LL * 65535, "%s: L=%d is too many tokens for one launch", fn, L);
   AttnArgs a{};

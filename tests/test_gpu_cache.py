@@ -163,6 +163,80 @@ def test_later_tokens_do_not_reach_earlier_ones(ns2lib, D, i4, fp16):
     assert not torch.isfinite(got[0, bad: bad + window]).any(-1).any(), "a visible NaN was lost"
 
 
+def attend64(q, pos, cache, window, sinks):
+    """R.attention over whole batches; what nobody sees has no part in cache.value."""
+    B, L, H, D = q.shape
+    p, j = pos.long()[:, :, None], torch.arange(cache.cap, device=DEV)
+    seen = (j <= p) & (p < cache.cap)
+    if window:
+        seen = seen & ((j < sinks) | (j > p - window))
+    k, v = (cache.value[n].permute(0, 2, 1, 3) for n in "kv")  # [B, KH, cap, D]
+    qg = q.reshape(B, L, cache.KH, H // cache.KH, D).permute(0, 2, 3, 1, 4)
+    m = seen[:, None, None]
+
+    def back(t):
+        return t.permute(0, 3, 1, 2, 4).reshape(B, L, H, -1)
+
+    s = torch.where(m, qg @ k[:, :, None].transpose(-1, -2).contiguous() / math.sqrt(D), -math.inf)
+    size = torch.where(m, qg.abs() @ k[:, :, None].abs().transpose(-1, -2).contiguous() / math.sqrt(D), 0.0).amax(-1, keepdim=True)
+    o = torch.softmax(s, -1) @ v[:, :, None]
+    vmax = v.abs().amax((2, 3))[:, :, None, None, None].expand_as(size)
+    return back(o), back(vmax), back(size), seen.sum(-1)[:, :, None, None].double()
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("B,L,H,KH,D", [(8, 140, 16, 16, 96), (16, 300, 8, 2, 64), (20, 270, 6, 2, 128), (43, 70, 4, 1, 256), (24, 150, 16, 8, 96)])
+def test_batches_of_prompts(ns2lib, B, L, H, KH, D, i4, fp16):
+    """Enough columns for every block size; sequences of unequal lengths, some without a token, rows nobody sees poisoned."""
+    cap = L + 90
+    spans = [((37 * b) % 90, (L, L - 1, 0, 1, 64, L // 2)[b % 6]) for b in range(B)]
+    pos = positions(spans, L)
+    rnd = gen(B + D)
+    q = rnd(B, L, H, D)
+    qd = (q.half() if fp16 else q).double()
+    for window, sinks in ((0, 0), (70, 3)):
+        cache = Cache(rnd, B, cap, KH, D, i4)
+        for b, (s, n) in enumerate(spans):
+            cache.poison(b, slice(s + n, None))
+            if window and s - window + 1 > sinks:
+                cache.poison(b, slice(sinks, s - window + 1))
+        got = attend(ns2lib, cache, q, pos, window, sinks, fp16)
+        ref, vmax, smax, n = attend64(qd, pos, cache, window, sinks)
+        live = (pos >= 0) & (pos < cap)
+        assert (got[~live] == 7).all(), "padding rows were written"
+        bound = R.attention_bound(ref, vmax, smax, n, D, fp16)[live]
+        err = (got[live].double() - ref[live]).abs()
+        print(f"[parity] {B}x{L} {H}/{KH}x{D} i4={i4} fp16={fp16}: largest error / bound {(err / bound).max().item():.3f}", flush=True)
+        assert torch.isfinite(got[live]).all() and (err <= bound).all()
+        # what enters at the token of row 50 shows in the rows that see it, and in no others
+        for b, (s, n) in enumerate(spans):
+            if n > 50:
+                cache.poison(b, slice(s + 50, s + 53))
+        bad = attend(ns2lib, cache, q, pos, window, sinks, fp16)
+        row = torch.arange(L, device=DEV)
+        far = row < 50
+        if window:
+            far = far | (row >= 52 + window)
+        assert torch.equal(bad[:, far], got[:, far])
+        hit = live & (row >= 52) & ((row < 51 + window) if window else True)  # (of rows 50 to 52, the third is finite)
+        assert not torch.isfinite(bad[hit]).any()
+
+
+@pytest.mark.parametrize("L", [3, 80])
+@pytest.mark.parametrize("D", [64, 256])
+def test_queries_of_any_magnitude(ns2lib, D, L):
+    """fp32 queries far below and beyond fp16's range, each head with its own; the scale takes the large ones back."""
+    rnd = gen(D + L)
+    pos = positions([(60, L), (0, L)], L)
+    cache = Cache(rnd, 2, 160, 2, D, False)
+    q = rnd(2, L, 4, D)
+    for h, f in ((0, 1e-20), (1, 1e-3), (2, 1.0), (3, 1e4)):
+        q[:, :, h] *= f
+    for scale, f in ((1 / math.sqrt(D), 1.0), (1e-25, 1e24), (1e20, 1e-21)):
+        check(attend(ns2lib, cache, q * f, pos, 0, 0, False, scale=scale), q * f, pos, cache, 0, 0, False, f"D={D} x {f}", scale=scale)
+
+
 @pytest.mark.parametrize("i4", [False, True])
 @pytest.mark.parametrize("L", [1, 40])
 def test_any_positions(ns2lib, L, i4):
@@ -404,6 +478,46 @@ def test_queries_in_place(ns2lib):
     assert torch.equal(y[:, : H * D], q) and torch.equal(y[:, H * D:], x[:, H * D:])
 
 
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("H,KH,D", [(8, 2, 64), (4, 4, 96), (6, 2, 128), (4, 1, 256)])
+def test_long_documents(ns2lib, H, KH, D, i4, fp16):
+    """Thousands of tokens in one call (several heads per lane group) hold what calls of 200 tokens write, bit for bit;
+    queries in place too."""
+    heads, per = H + 2 * KH, 256 // D
+    L = 16384 * per // (2 * heads) + 77
+    cap = L + 9
+    rnd = gen(D)
+    x = rnd(2 * L, heads * D)
+    pos = positions([(9, L), (0, L - 50)], L)
+    w, cs = 1 + 0.2 * rnd(D), R.rope_table(cap, D).to(DEV)
+    a = dict(i4=i4, fp16=fp16, wq=w, wk=w, cs=cs, rope_rows=cap - 5, fill=1)
+    got = write(ns2lib, x, pos, H, KH, D, cap, **a)
+    seq = x.reshape(2, L, -1)
+    want = None
+    for i in range(0, L, 200):
+        part = write(ns2lib, seq[:, i: i + 200].reshape(-1, heads * D).contiguous(), pos[:, i: i + 200].contiguous(), H, KH, D, cap, **a)
+        if want is None:
+            want = {n: t.clone() for n, t in part.items() if n != "q"}
+        n = min(200, L - i)
+        assert torch.equal(got["q"].reshape(2, L, -1)[:, i: i + n], part["q"].reshape(2, n, -1))
+        for b in range(2):
+            at = pos[b, i: i + n].long()
+            at = at[at >= 0]
+            for name in want:
+                want[name][b, at] = part[name][b, at]
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+    if not fp16:
+        y, k, v = x.clone(), *(torch.zeros(2, cap, KH * D, dtype=torch.float16, device=DEV) for _ in "kv")
+        ns2lib.head_norm_cache(y, pos, y, k, v, batch=2, L=L, H=H, KH=KH, D=D, ldx=heads * D, ldq=heads * D, cap=cap, ldkv=KH * D,
+                               kvBatch=cap * KH * D, w_q=w, w_k=w, cs=cs, sin_off=cs.numel() // 2, rope_rows=cap - 5)
+        torch.cuda.synchronize()
+        live = (pos >= 0).flatten()
+        assert torch.equal(y[live, : H * D], got["q"][live, : H * D]) and torch.equal(y[:, H * D:], x[:, H * D:])
+        assert torch.equal(y[~live], x[~live])
+
+
 # ---- graphs, streams, refusals ----------------------------------------------------------------------
 
 @pytest.mark.parametrize("i4", [False, True])
@@ -459,7 +573,8 @@ BASE = dict(batch=1, L=1, H=4, KH=2, D=64, cap=64, ldkv=128, kvBatch=64 * 128, l
 @pytest.mark.parametrize("change", [dict(D=80), dict(D=32), dict(D=512), dict(H=3), dict(KH=0), dict(H=0), dict(cap=0), dict(ldq=255),
                                     dict(ldq=258), dict(ldkv=120), dict(ldkv=132), dict(kvBatch=-8), dict(kvBatch=8196), dict(q_fmt=2),
                                     dict(window=-1), dict(sinks=-1), dict(ldo=128), dict(ldo=257), dict(k=None), dict(v=None),
-                                    dict(pos=None), dict(q=None), dict(o=None), dict(vg=None), dict(k=8), dict(q=4), dict(o=4)])
+                                    dict(pos=None), dict(q=None), dict(o=None), dict(vg=None), dict(k=8), dict(q=4), dict(o=4), dict(cap=(1 << 30) + 1),
+                                    dict(batch=1 << 22), dict(batch=1 << 30, L=1 << 30), dict(L=1 << 22)])
 def test_attention_refusals(ns2lib, change):
     """Refused on the host, before any launch: the output keeps what it held."""
     import ns2
@@ -486,7 +601,8 @@ def test_attention_refusals(ns2lib, change):
 
 @pytest.mark.parametrize("change", [dict(D=48), dict(H=5), dict(ldx=500), dict(ldx=514), dict(x=4), dict(x=None), dict(wk=4), dict(cs=4),
                                     dict(sin_off=2), dict(sin_off=-4), dict(rope_rows=-1), dict(batch=2, kvBatch=64), dict(kvBatch=8196),
-                                    dict(kg=None), dict(k=2), dict(ldq=250)])
+                                    dict(kg=None), dict(k=2), dict(ldq=250), dict(cap=(1 << 30) + 1),
+                                    dict(batch=1 << 30, L=1 << 30, kvBatch=64 * 128)])
 def test_write_refusals(ns2lib, change):
     import ns2
 
