@@ -113,7 +113,7 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
   half_t sc[PD][CT];
   auto load = [&](int s, int chunk) {
     int k = chunk * kChunk + 32 * g;
-    k = k < p.K ? k : 0;  // (a step past K is not used)
+    k = k < p.K ? k : 0;  // (a step past K meets zeros of x)
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       w[s][c] = *reinterpret_cast<const uint4*>(wr[c] + k / 2);
@@ -139,7 +139,7 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
 
   for (int k0 = 0; k0 < p.K; k0 += p.slab) {
     const int ks = p.K - k0 < p.slab ? p.K - k0 : p.slab;
-    const int n8 = ks / 8, items = rows * n8;
+    const int n8 = (ks + kChunk - 1) / kChunk * (kChunk / 8), items = rows * n8;  // (zeros behind K, to the end of its chunk)
     half8_t* lo_s = x_s + items;
     const int first = k0 / kChunk + (WK == 1 ? 0 : wave), last = (k0 + ks + kChunk - 1) / kChunk;
 #pragma unroll
@@ -149,7 +149,8 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
     if constexpr (A16) {
       for (int u = threadIdx.x; u < items; u += 64 * kWaves) {
         const int r = u / n8, k8 = u - r * n8;
-        const half8_t v = *reinterpret_cast<const half8_t*>(static_cast<const half_t*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8);
+        half8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (8 * k8 < ks) v = *reinterpret_cast<const half8_t*>(static_cast<const half_t*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8);
         x_s[k8 * rows + r] = half8_t{v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
       }
     } else {
@@ -160,7 +161,7 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
       for (int i = 0; i < NI; ++i) {
         const int u = threadIdx.x + 64 * kWaves * i, r = u / n8, k8 = u - r * n8;
         x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (u < items) {
+        if (u < items && 8 * k8 < ks) {
           const float* a = static_cast<const float*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8;
           x[i][0] = *reinterpret_cast<const float4*>(a);
           x[i][1] = *reinterpret_cast<const float4*>(a + 4);
@@ -220,7 +221,7 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
             t[c][1] = w[sl][c].y;
             t[c][2] = w[sl][c].z;
             t[c][3] = w[sl][c].w;
-            const float f = (float)sc[sl][c];
+            const float f = ch * kChunk + 32 * g < p.K ? (float)sc[sl][c] : 0.f;
             uint32_t a = __builtin_bit_cast(uint32_t, f), b = a;
             permlane32_swap(a, b);  // the scales of steps 0, 1 | 2, 3
             uint32_t a1 = a, b1 = b;
@@ -238,25 +239,23 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
           float4_t d[RT][CT];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            if (ch * kChunk + 32 * j < k0 + ks) {  // uniform
-              half8_t xh[RT], xl[RT];
+            half8_t xh[RT], xl[RT];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+              xh[i] = x_s[(base + 4 * j) * rows + arow[i]];
+              if constexpr (!A16) xl[i] = lo_s[(base + 4 * j) * rows + arow[i]];
+            }
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+              const half8_t q = codes8(t[c][j]);
 #pragma unroll
               for (int i = 0; i < RT; ++i) {
-                xh[i] = x_s[(base + 4 * j) * rows + arow[i]];
-                if constexpr (!A16) xl[i] = lo_s[(base + 4 * j) * rows + arow[i]];
-              }
+                if (j % SG == 0) d[i][c] = float4_t{0.f, 0.f, 0.f, 0.f};
+                d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[i], q, d[i][c], 0, 0, 0);
+                if constexpr (!A16) d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[i], q, d[i][c], 0, 0, 0);
+                if (j % SG == SG - 1) {
 #pragma unroll
-              for (int c = 0; c < CT; ++c) {
-                const half8_t q = codes8(t[c][j]);
-#pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                  if (j % SG == 0) d[i][c] = float4_t{0.f, 0.f, 0.f, 0.f};
-                  d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[i], q, d[i][c], 0, 0, 0);
-                  if constexpr (!A16) d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[i], q, d[i][c], 0, 0, 0);
-                  if (j % SG == SG - 1) {
-#pragma unroll
-                    for (int r = 0; r < NR; ++r) acc[i][c][r] = fmaf(s[c][j], d[i][c][r], acc[i][c][r]);
-                  }
+                  for (int r = 0; r < NR; ++r) acc[i][c][r] = fmaf(s[c][j], d[i][c][r], acc[i][c][r]);
                 }
               }
             }
@@ -319,7 +318,7 @@ template <bool A16, int SG, int RT, int NR, int CT, int WK>
 void launch_i4(I4Args p, hipStream_t s) {
   const int rows = p.M < 16 * RT ? p.M : 16 * RT, per = rows * (A16 ? 2 : 4);  // bytes of a column of k
   p.slab = slab_bytes<A16, RT>() / per / kChunk * kChunk;
-  if (p.slab > p.K) p.slab = p.K;
+  if (p.slab > p.K) p.slab = (p.K + kChunk - 1) / kChunk * kChunk;
   constexpr int kWaves = waves<WK>();
   const size_t red = WK > 1 ? sizeof(float) * kWaves * RT * CT * NR * 64 : 0;
   const size_t lds = std::max<size_t>((size_t)p.slab * per, red);
