@@ -77,25 +77,22 @@ template <int WK>
 constexpr int waves() {
   return WK == 16 ? 16 : 4;
 }
-template <bool A16, int RT>
-constexpr int slab_bytes() {
-  return A16 && RT > 1 ? 32 * 1024 : 48 * 1024;
-}
+constexpr int kSlabBytes = 48 * 1024;
 
-// A block takes 16 RT rows and, with WK = 1, 64 CT columns (16 CT per wave) over all of K; with WK = 4, 16 CT
-// columns whose chunks its waves take in turn and add up at the end. NR: result registers in use (4 NR rows of
-// each 16). SG: 32-column steps per group. The block's rows of x go to LDS a slab of p.slab columns at a time:
-// operand (step, lane group, row), `rows` rows, hi then lo.
-template <bool A16, int SG, int RT, int NR, int CT, int WK>
+// A block takes 16 rows and, with WK = 1, 64 CT columns (16 CT per wave) over all of K; with WK = 4 or 16, 16 CT
+// columns whose chunks its WK waves take in turn and add up at the end. NR: result registers in use (4 NR rows).
+// SG: 32-column steps per group. The block's rows of x go to LDS a slab of p.slab columns at a time: operand
+// (step, lane group, row), `rows` rows, hi then lo.
+template <bool A16, int SG, int NR, int CT, int WK>
 __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p) {
   constexpr int kWaves = waves<WK>();
   extern __shared__ __attribute__((aligned(16))) char smem[];
   half8_t* x_s = reinterpret_cast<half8_t*>(smem);
-  __shared__ uint32_t top_s[16 * RT];
+  __shared__ uint32_t top_s[16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c16 = lane & 15, g = lane >> 4;
-  const int m0 = blockIdx.y * (16 * RT);
-  const int rows = p.M - m0 < 16 * RT ? p.M - m0 : 16 * RT;
+  const int m0 = blockIdx.y * 16;
+  const int rows = p.M - m0 < 16 ? p.M - m0 : 16;
   const int n0 = (WK == 1 ? blockIdx.x * kWaves + wave : blockIdx.x) * (16 * CT);
   const int kb = p.K / 2, kg = p.K / (32 * SG);
 
@@ -121,21 +118,13 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
     }
   };
 
-  float tot[RT][CT][NR];
+  float tot[CT][NR];
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+  for (int c = 0; c < CT; ++c)
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-      for (int r = 0; r < NR; ++r) tot[i][c][r] = 0.f;
+    for (int r = 0; r < NR; ++r) tot[c][r] = 0.f;
 
-  // this lane's rows: of the A operand, and of the results
-  int arow[RT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int r = 16 * i + (c16 >> 2) + 4 * (c16 & 3);
-    arow[i] = r < rows ? r : rows - 1;
-  }
+  const int ar = (c16 >> 2) + 4 * (c16 & 3), arow = ar < rows ? ar : rows - 1;  // this lane's row of the A operand
 
   for (int k0 = 0; k0 < p.K; k0 += p.slab) {
     const int ks = p.K - k0 < p.slab ? p.K - k0 : p.slab;
@@ -154,7 +143,7 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
         x_s[k8 * rows + r] = half8_t{v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
       }
     } else {
-      constexpr int NI = (slab_bytes<A16, RT>() / 32 + 64 * kWaves - 1) / (64 * kWaves);  // pieces of 8 columns per thread
+      constexpr int NI = (kSlabBytes / 32 + 64 * kWaves - 1) / (64 * kWaves);  // pieces of 8 columns per thread
       float4 x[NI][2];
       for (int u = threadIdx.x; u < rows; u += 64 * kWaves) top_s[u] = 0u;
 #pragma unroll
@@ -201,13 +190,11 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
     }
     __syncthreads();
 
-    float acc[RT][CT][NR];
+    float acc[CT][NR];
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
-      for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int r = 0; r < NR; ++r) acc[i][c][r] = 0.f;
+      for (int r = 0; r < NR; ++r) acc[c][r] = 0.f;
     for (int chunk = first; chunk < last; chunk += PD * WK) {
 #pragma unroll
       for (int sl = 0; sl < PD; ++sl) {
@@ -236,27 +223,21 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
           for (int c = 0; c < CT; ++c) transpose_rows(t[c]);
           if (ch + PD * WK < last) load(sl, ch + PD * WK);
           const int base = (ch * kChunk - k0) / 8 + g;
-          float4_t d[RT][CT];
+          float4_t d[CT];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            half8_t xh[RT], xl[RT];
-#pragma unroll
-            for (int i = 0; i < RT; ++i) {
-              xh[i] = x_s[(base + 4 * j) * rows + arow[i]];
-              if constexpr (!A16) xl[i] = lo_s[(base + 4 * j) * rows + arow[i]];
-            }
+            const half8_t xh = x_s[(base + 4 * j) * rows + arow];
+            half8_t xl;
+            if constexpr (!A16) xl = lo_s[(base + 4 * j) * rows + arow];
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
               const half8_t q = codes8(t[c][j]);
+              if (j % SG == 0) d[c] = float4_t{0.f, 0.f, 0.f, 0.f};
+              d[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, q, d[c], 0, 0, 0);
+              if constexpr (!A16) d[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, q, d[c], 0, 0, 0);
+              if (j % SG == SG - 1) {
 #pragma unroll
-              for (int i = 0; i < RT; ++i) {
-                if (j % SG == 0) d[i][c] = float4_t{0.f, 0.f, 0.f, 0.f};
-                d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[i], q, d[i][c], 0, 0, 0);
-                if constexpr (!A16) d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[i], q, d[i][c], 0, 0, 0);
-                if (j % SG == SG - 1) {
-#pragma unroll
-                  for (int r = 0; r < NR; ++r) acc[i][c][r] = fmaf(s[c][j], d[i][c][r], acc[i][c][r]);
-                }
+                for (int r = 0; r < NR; ++r) acc[c][r] = fmaf(s[c][j], d[c][r], acc[c][r]);
               }
             }
           }
@@ -264,36 +245,31 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
       }
     }
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        float back = 1.f;
-        if constexpr (!A16) {
-          const int row = 16 * i + g + 4 * r;
-          back = ldexpf(1.f, -i4_up(__builtin_bit_cast(float, top_s[row < rows ? row : rows - 1])));
-        }
-#pragma unroll
-        for (int c = 0; c < CT; ++c) tot[i][c][r] = fmaf(acc[i][c][r], back, tot[i][c][r]);
+    for (int r = 0; r < NR; ++r) {
+      float back = 1.f;
+      if constexpr (!A16) {
+        const int row = g + 4 * r;
+        back = ldexpf(1.f, -i4_up(__builtin_bit_cast(float, top_s[row < rows ? row : rows - 1])));
       }
+#pragma unroll
+      for (int c = 0; c < CT; ++c) tot[c][r] = fmaf(acc[c][r], back, tot[c][r]);
+    }
   }
 
   if constexpr (WK > 1) {
-    float* red = reinterpret_cast<float*>(smem);  // [wave][i][c][r][lane]
-    constexpr int T = RT * CT * NR;
+    float* red = reinterpret_cast<float*>(smem);  // [wave][c][r][lane]
+    constexpr int T = CT * NR;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
-      for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int r = 0; r < NR; ++r) red[(wave * T + (i * CT + c) * NR + r) * 64 + lane] = tot[i][c][r];
+      for (int r = 0; r < NR; ++r) red[(wave * T + c * NR + r) * 64 + lane] = tot[c][r];
     __syncthreads();
     for (int u = wave; u < T; u += kWaves) {
       float sum = 0.f;
 #pragma unroll
       for (int v = 0; v < kWaves; ++v) sum += red[(v * T + u) * 64 + lane];
-      const int r = u % NR, c = u / NR % CT, i = u / NR / CT;
-      const int m = m0 + 16 * i + g + 4 * r, n = n0 + 16 * c + c16;
+      const int m = m0 + g + 4 * (u % NR), n = n0 + 16 * (u / NR) + c16;
       if (m < m0 + rows && n < p.N) store_i4(p, m, n, sum, p.bias ? p.bias[n] : 0.f, p.gate ? p.gate[p.gOff + n] : 1.f);
     }
   } else {
@@ -303,65 +279,54 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
       if (n < p.N) {
         const float bi = p.bias ? p.bias[n] : 0.f, gt = p.gate ? p.gate[p.gOff + n] : 1.f;
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            const int m = m0 + 16 * i + g + 4 * r;
-            if (m < m0 + rows) store_i4(p, m, n, tot[i][c][r], bi, gt);
-          }
+        for (int r = 0; r < NR; ++r) {
+          const int m = m0 + g + 4 * r;
+          if (m < m0 + rows) store_i4(p, m, n, tot[c][r], bi, gt);
+        }
       }
     }
   }
 }
 
-template <bool A16, int SG, int RT, int NR, int CT, int WK>
-void launch_i4(I4Args p, hipStream_t s) {
-  const int rows = p.M < 16 * RT ? p.M : 16 * RT, per = rows * (A16 ? 2 : 4);  // bytes of a column of k
-  p.slab = slab_bytes<A16, RT>() / per / kChunk * kChunk;
+template <bool A16, int SG, int NR, int CT, int WK>
+void launch_rows(I4Args p, hipStream_t s) {
+  const int rows = p.M < 16 ? p.M : 16, per = rows * (A16 ? 2 : 4);  // bytes of a column of k
+  p.slab = kSlabBytes / per / kChunk * kChunk;
   if (p.slab > p.K) p.slab = (p.K + kChunk - 1) / kChunk * kChunk;
   constexpr int kWaves = waves<WK>();
-  const size_t red = WK > 1 ? sizeof(float) * kWaves * RT * CT * NR * 64 : 0;
+  const size_t red = WK > 1 ? sizeof(float) * kWaves * CT * NR * 64 : 0;
   const size_t lds = std::max<size_t>((size_t)p.slab * per, red);
   const int cols = 16 * CT * (WK == 1 ? kWaves : 1);
-  const dim3 grid((unsigned)((p.N + cols - 1LL) / cols), (unsigned)((p.M + 16 * RT - 1) / (16 * RT)));
-  linear_i4_kernel<A16, SG, RT, NR, CT, WK><<<grid, 64 * kWaves, lds, s>>>(p);
+  const dim3 grid((unsigned)((p.N + cols - 1LL) / cols), (unsigned)((p.M + 15) / 16));
+  linear_i4_kernel<A16, SG, NR, CT, WK><<<grid, 64 * kWaves, lds, s>>>(p);
+}
+template <bool A16, int SG, int CT, int WK>
+void launch_i4(const I4Args& p, hipStream_t s) {
+  if (p.M <= 4) launch_rows<A16, SG, 1, CT, WK>(p, s);
+  else if (p.M <= 8) launch_rows<A16, SG, 2, CT, WK>(p, s);
+  else launch_rows<A16, SG, 4, CT, WK>(p, s);
 }
 
-// us, fp16 x and 32-column groups unless said otherwise:
-//  - many rows: 32 x 128 blocks from 4096 (fp32 x: 2048) 16 x 16 tiles on, else 16 x 16 blocks whose waves split
-//    K (256 x 4096 x 640 12.4, 32 x 4096 x 640 4.4; as the other 12.7, 5.7);
-//  - up to 16 rows and 65536 columns: a wave per 16 columns (fp32 x or more than 4 rows: 32, since the rows'
-//    operands then cost more) over all of K, each with loads coming for two to four chunks (1 x 262144 x 640
-//    18.2, with 64 columns per wave 23.9, split over K 22.3; 1 x 65536 x 4096 34.5, 42.8, 33.7);
-//  - few columns: K over the sixteen waves of a block where that is one block per CU or two (1 x 1536 x 640 fp32
-//    3.6, over four 4.0; 1 x 8192 x 1536 4.1, 4.7), 32 columns each where fp32 rows would be read by 512 blocks
-//    (5 x 8192 x 1536 fp32 5.6, with 16 columns 7.5, over four waves 6.7);
-//  - else over four waves, 32 columns each (8 x 16384 x 4096 fp32 26.4, with 16 columns 38.1; up to four fp16
-//    rows cost too little for that: 2 x 20000 x 640 4.3, 4.0).
+// By the number of 16 x 16 tiles of the output (us, "a | b": fp16 | fp32 x):
+//  - many tiles: all of K in a wave of 32 columns, loads two chunks ahead (256 x 4096 x 640 10.1 | 12.6,
+//    over four waves 11.7 | 22.3; 12 x 32768 x 2048 16.7 | 19.3, 19.5 | 25.9); with up to four fp16 rows, whose
+//    products cost least, 16 columns and loads four chunks ahead (1 x 262144 x 640 17.6, with 32 columns 19.6);
+//  - few tiles and a K that gives sixteen waves work: over sixteen waves (1 x 8192 x 1536 4.2 | 4.8, over
+//    four 4.6 | 4.9; 16 x 8192 x 1536 5.8 | 9.7, 7.0 | 12.0), of 16 columns up to one block per CU or where rows
+//    cost least (16 x 4096 x 1536 fp32 8.9, with 32 columns 9.6), else of 32 (16 x 8192 x 1536 fp32 9.7, with 16 16.0);
+//  - between: over four waves of 32 columns (8 x 16384 x 4096 fp32 25.5, with 16 columns 35.6; in one wave 30.2).
 template <bool A16, int SG>
 void choose_i4(const I4Args& p, hipStream_t s) {
-  const long long tiles = (p.N + 15) / 16, units = tiles * ((p.M + 15) / 16);
-  if (p.M > 16 && units >= (A16 ? 4096 : 2048)) {
-    launch_i4<A16, SG, 2, 4, 2, 1>(p, s);
-  } else if (p.M <= 16 && tiles >= 4096) {
-    if (p.M <= 4) launch_i4<A16, SG, 1, 1, A16 ? 1 : 2, 1>(p, s);
-    else if (p.M <= 8) launch_i4<A16, SG, 1, 2, 2, 1>(p, s);
-    else launch_i4<A16, SG, 1, 4, 2, 1>(p, s);
-  } else if (p.K > 4 * kChunk && units <= (A16 ? 512 : 256)) {
-    if (p.M <= 4) launch_i4<A16, SG, 1, 1, 1, 16>(p, s);
-    else if (p.M <= 8) launch_i4<A16, SG, 1, 2, 1, 16>(p, s);
-    else launch_i4<A16, SG, 1, 4, 1, 16>(p, s);
-  } else if (!A16 && p.K > 4 * kChunk && units <= 512) {
-    if constexpr (!A16) {
-      if (p.M <= 4) launch_i4<A16, SG, 1, 1, 2, 16>(p, s);
-      else if (p.M <= 8) launch_i4<A16, SG, 1, 2, 2, 16>(p, s);
-      else launch_i4<A16, SG, 1, 4, 2, 16>(p, s);
+  const long long tiles = (p.N + 15) / 16 * ((p.M + 15LL) / 16);
+  const bool light = A16 && p.M <= 4, deep = p.K > 4 * kChunk;
+  if (tiles >= (A16 ? 2048 : 1536)) {
+    if constexpr (A16) {
+      if (light) return launch_rows<A16, SG, 1, 1, 1>(p, s);
     }
-  } else {
-    if (p.M <= 4) launch_i4<A16, SG, 1, 1, A16 ? 1 : 2, 4>(p, s);
-    else if (p.M <= 8) launch_i4<A16, SG, 1, 2, 2, 4>(p, s);
-    else launch_i4<A16, SG, 1, 4, 2, 4>(p, s);
-  }
+    launch_i4<A16, SG, 2, 1>(p, s);
+  } else if (deep && tiles <= (light ? 512 : 256)) launch_i4<A16, SG, 1, 16>(p, s);
+  else if (deep && tiles <= 512) launch_i4<A16, SG, 2, 16>(p, s);
+  else launch_i4<A16, SG, 2, 4>(p, s);
 }
 
 // One thread per group: the group's largest magnitude a goes to code 1 or 15 with step
