@@ -16,67 +16,77 @@ using namespace ns2cache;
 namespace {
 
 constexpr int kTile = 64;  // keys
-constexpr int kThreads = 512;
-constexpr int kHalf = 256;  // threads that bring K, and V
 
-// What one thread brings of a tile from memory to LDS: NK pieces of 8 dimensions of K rows, or one block of
-// 8 keys x VD dimensions of V.
+constexpr int kWaves = 8, kThreads = 64 * kWaves, kGroups = kWaves / 2;  // (groups of columns)
+
+// What one of the T threads brings of a tile from memory to LDS: NK pieces of 8 dimensions of K rows, and NV blocks of
+// 4 keys x VD dimensions of V.
 template <int D, bool I4>
 struct Stage {
-  static constexpr int C = D / 8, NK = kTile * C / kHalf;  // 8-dimension pieces of a row; of K per thread
-  static constexpr int VD = D == 256 ? 8 : D >= 96 ? 4 : 2, VC = D / VD;
-  static constexpr int NR = I4 ? 8 : NK * 4 > 4 * VD ? NK * 4 : 4 * VD;
-  static_assert(kTile * C % kHalf == 0 && 8 * VC <= kHalf && NK <= 8, "thread shares");
-  uint32_t raw[NR], group[I4 ? 8 : 1];
+  static constexpr int T = kThreads;
+  static constexpr int C = D / 8, KU = kTile * C, NK = (KU + T - 1) / T;  // pieces of a K row, of a tile, of a thread
+  static constexpr int VD = D == 256 ? 8 : D >= 96 ? 4 : 2, VC = D / VD, VU = kTile / 4 * VC, NV = (VU + T - 1) / T;
+  uint32_t k[NK][I4 ? 1 : 4], kg[I4 ? NK : 1], v[NV][I4 ? 4 : 2 * VD], vg[I4 ? NV : 1][4];
 
-  __device__ __forceinline__ void load_k(const AttnArgs& a, long long base, const Tile& t, int tid) {
-    const char* rows = tile_rows(a.k, base, t.key0, a.ldkv, I4);
-    const half2_t* groups = I4 ? tile_groups(a.kg, base, t.key0, a.ldkv) : nullptr;
+  static __device__ __forceinline__ bool has_k(int u) { return KU % T == 0 || u < KU; }
+  static __device__ __forceinline__ bool has_v(int u) { return VU % T == 0 || u < VU; }
+  // Block u: four keys from 32 (q / 4) + 4 (q % 4) + 16 h on, where 2 q + h is the half fragment it goes to. (The two
+  // halves are neighbours, so that 16 lanes write 16 different 8-byte banks; the last threads start, since the first
+  // have a K piece more where T does not divide them.)
+  static __device__ __forceinline__ int block_of(int tid, int i) { return T - 1 - tid + T * i; }
+  static __device__ __forceinline__ int column_of(int u) { return (u >> 1) % VC; }
+  static __device__ __forceinline__ int q_of(int u) { return (u >> 1) / VC; }
+  static __device__ __forceinline__ int key_of(int u) { return 32 * (q_of(u) >> 2) + 4 * (q_of(u) & 3) + 16 * (u & 1); }
+
+  __device__ __forceinline__ void load(const AttnArgs& a, long long base, const Tile& t, int tid) {
     const int last = t.end - 1 - t.key0;
+    {
+      const char* rows = tile_rows(a.k, base, t.key0, a.ldkv, I4);
+      const half2_t* groups = I4 ? tile_groups(a.kg, base, t.key0, a.ldkv) : nullptr;
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const int u = tid + kHalf * i, key = min(u / C, last), c = u % C;
-      const uint32_t at = (uint32_t)(key * a.ldkv + 8 * c);
-      if constexpr (I4) {
-        raw[i] = *reinterpret_cast<const uint32_t*>(rows + at / 2);
-        group[i] = __builtin_bit_cast(uint32_t, groups[at / kGroup]);
-      } else {
-        const uint4 x = *reinterpret_cast<const uint4*>(rows + 2u * at);
-        raw[4 * i] = x.x;
-        raw[4 * i + 1] = x.y;
-        raw[4 * i + 2] = x.z;
-        raw[4 * i + 3] = x.w;
+      for (int i = 0; i < NK; ++i) {
+        const int u = tid + T * i;
+        if (!has_k(u)) continue;
+        const uint32_t at = (uint32_t)(min(u / C, last) * a.ldkv + 8 * (u % C));
+        if constexpr (I4) {
+          k[i][0] = *reinterpret_cast<const uint32_t*>(rows + at / 2);
+          kg[i] = __builtin_bit_cast(uint32_t, groups[at / kGroup]);
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4*>(rows + 2u * at);
+          k[i][0] = x.x;
+          k[i][1] = x.y;
+          k[i][2] = x.z;
+          k[i][3] = x.w;
+        }
       }
     }
-  }
-
-  __device__ __forceinline__ void load_v(const AttnArgs& a, long long base, const Tile& t, int tid) {
-    if (8 * VC < kHalf && tid >= 8 * VC) return;
     const char* rows = tile_rows(a.v, base, t.key0, a.ldkv, I4);
     const half2_t* groups = I4 ? tile_groups(a.vg, base, t.key0, a.ldkv) : nullptr;
-    const int last = t.end - 1 - t.key0;
-    const int c = tid % VC, q = tid / VC;  // q = 4 (tile half) + lane group
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int key = min(32 * (q >> 2) + 4 * (q & 3) + (j < 4 ? j : 12 + j), last);
-      const uint32_t at = (uint32_t)(key * a.ldkv + VD * c);
-      if constexpr (I4) {
-        raw[j] = VD == 8   ? *reinterpret_cast<const uint32_t*>(rows + at / 2)
-                 : VD == 4 ? *reinterpret_cast<const uint16_t*>(rows + at / 2)
-                           : *reinterpret_cast<const uint8_t*>(rows + at / 2);
-        group[j] = __builtin_bit_cast(uint32_t, groups[at / kGroup]);
-      } else if constexpr (VD == 8) {
-        const uint4 x = *reinterpret_cast<const uint4*>(rows + 2u * at);
-        raw[4 * j] = x.x;
-        raw[4 * j + 1] = x.y;
-        raw[4 * j + 2] = x.z;
-        raw[4 * j + 3] = x.w;
-      } else if constexpr (VD == 4) {
-        const uint2 x = *reinterpret_cast<const uint2*>(rows + 2u * at);
-        raw[2 * j] = x.x;
-        raw[2 * j + 1] = x.y;
-      } else {
-        raw[j] = *reinterpret_cast<const uint32_t*>(rows + 2u * at);
+    for (int i = 0; i < NV; ++i) {
+      const int u = block_of(tid, i);
+      if (!has_v(u)) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t at = (uint32_t)(min(key_of(u) + j, last) * a.ldkv + VD * column_of(u));
+        if constexpr (I4) {
+          v[i][j] = VD == 8   ? *reinterpret_cast<const uint32_t*>(rows + at / 2)
+                    : VD == 4 ? *reinterpret_cast<const uint16_t*>(rows + at / 2)
+                              : *reinterpret_cast<const uint8_t*>(rows + at / 2);
+          vg[i][j] = __builtin_bit_cast(uint32_t, groups[at / kGroup]);
+        } else if constexpr (VD == 8) {
+          const uint4 x = *reinterpret_cast<const uint4*>(rows + 2u * at);
+          v[i][4 * j] = x.x;
+          v[i][4 * j + 1] = x.y;
+          v[i][4 * j + 2] = x.z;
+          v[i][4 * j + 3] = x.w;
+        } else if constexpr (VD == 4) {
+          const uint2 x = *reinterpret_cast<const uint2*>(rows + 2u * at);
+          v[i][2 * j] = x.x;
+          v[i][2 * j + 1] = x.y;
+        } else {
+          v[i][j] = *reinterpret_cast<const uint32_t*>(rows + 2u * at);
+        }
       }
     }
   }
@@ -85,49 +95,54 @@ struct Stage {
   __device__ __forceinline__ void store_k(half8_t* ksm, int tid) const {
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-      const int u = tid + kHalf * i, key = u / C, c = u % C;
+      const int u = tid + T * i, key = u / C, c = u % C;
+      if (!has_k(u)) continue;
       half8_t x;
-      if constexpr (I4) x = dequant8(raw[i], __builtin_bit_cast(half2_t, group[i]));
-      else x = __builtin_bit_cast(half8_t, make_uint4(raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]));
+      if constexpr (I4) x = dequant8(k[i][0], __builtin_bit_cast(half2_t, kg[i]));
+      else x = __builtin_bit_cast(half8_t, make_uint4(k[i][0], k[i][1], k[i][2], k[i][3]));
       ksm[((key >> 4) * (D / 32) + (c >> 2)) * 64 + (c & 3) * 16 + ((key ^ c) & 15)] = x;
     }
   }
 
   // V fragment (step t, tile half): lane (dimension % 16, grp) holds the eight keys of grp. Returns NaN if a value
   // is not finite and `check` is set.
+  static __device__ __forceinline__ int v_slot(int t, int d) { return d ^ (t & (VD - 1)) ^ ((d >> 3) * (VD / 2)); }
   __device__ __forceinline__ half2_t store_v(half8_t* vsm, int tid, bool check) const {
     half2_t z = {0.f, 0.f};
-    if (8 * VC < kHalf && tid >= 8 * VC) return z;
-    const int c = tid % VC, q = tid / VC;
-    uint32_t r[VD][4];  // [dimension][key pair]
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (I4) {
-        const half2_t s = __builtin_bit_cast(half2_t, pair_lo(group[2 * j], group[2 * j + 1]));
-        const half2_t o = __builtin_bit_cast(half2_t, pair_hi(group[2 * j], group[2 * j + 1]));
+    for (int i = 0; i < NV; ++i) {
+      const int u = block_of(tid, i), c = column_of(u), q = q_of(u);
+      if (!has_v(u)) continue;
+      uint32_t r[VD][2];  // [dimension][key pair]
 #pragma unroll
-        for (int h = 0; h < (VD + 3) / 4; ++h) {
-          uint32_t x[4];
-          dequant4(h ? pair_hi(raw[2 * j], raw[2 * j + 1]) : pair_lo(raw[2 * j], raw[2 * j + 1]), s, o, x);
+      for (int j = 0; j < 2; ++j) {
+        if constexpr (I4) {
+          const half2_t s = __builtin_bit_cast(half2_t, pair_lo(vg[i][2 * j], vg[i][2 * j + 1]));
+          const half2_t o = __builtin_bit_cast(half2_t, pair_hi(vg[i][2 * j], vg[i][2 * j + 1]));
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (4 * h + e < VD) r[4 * h + e][j] = x[e];
-        }
-      } else {
+          for (int h = 0; h < (VD + 3) / 4; ++h) {
+            uint32_t x[4];
+            dequant4(h ? pair_hi(v[i][2 * j], v[i][2 * j + 1]) : pair_lo(v[i][2 * j], v[i][2 * j + 1]), s, o, x);
 #pragma unroll
-        for (int e = 0; e < VD / 2; ++e) {
-          const uint32_t x = raw[2 * j * (VD / 2) + e], y = raw[(2 * j + 1) * (VD / 2) + e];
-          r[2 * e][j] = pair_lo(x, y);
-          r[2 * e + 1][j] = pair_hi(x, y);
+            for (int e = 0; e < 4; ++e)
+              if (4 * h + e < VD) r[4 * h + e][j] = x[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VD / 2; ++e) {
+            const uint32_t x = v[i][2 * j * (VD / 2) + e], y = v[i][(2 * j + 1) * (VD / 2) + e];
+            r[2 * e][j] = pair_lo(x, y);
+            r[2 * e + 1][j] = pair_hi(x, y);
+          }
         }
       }
-    }
-    const int t = VD * c >> 4;
+      const int t = VD * c >> 4;
 #pragma unroll
-    for (int e = 0; e < VD; ++e) {
-      const half8_t x = __builtin_bit_cast(half8_t, make_uint4(r[e][0], r[e][1], r[e][2], r[e][3]));
-      if (check) spot(x, z);
-      vsm[(t * 2 + (q >> 2)) * 64 + (q & 3) * 16 + (((VD * c & 15) + e) ^ (t & (VD - 1)))] = x;
+      for (int e = 0; e < VD; ++e) {
+        const uint2 x = make_uint2(r[e][0], r[e][1]);
+        if (check) spot(__builtin_bit_cast(half4_t, x), z);
+        reinterpret_cast<uint2*>(vsm + (t * 2 + (q >> 2)) * 64 + (q & 3) * 16 + v_slot(t, (VD * c & 15) + e))[u & 1] = x;
+      }
     }
     return z;
   }
@@ -135,13 +150,14 @@ struct Stage {
 
 template <int D, bool I4, bool F32, int CT>
 __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
-  constexpr int DT = D / 16, QT = D / 32, VD = Stage<D, I4>::VD;
-  constexpr int kFrags = 4 * QT + 2 * DT, kMerge = 4 * CT * (DT + 1);  // KB of a tile; of the second halves' sums
+  typedef Stage<D, I4> Bring;
+  constexpr int DT = D / 16, QT = D / 32, kColumns = 16 * CT * kGroups;
+  constexpr int kFrags = 4 * QT + 2 * DT, kMerge = kGroups * CT * (DT + 1);  // KB of a tile; of the second halves' sums
   __shared__ __attribute__((aligned(16))) half8_t smem[(2 * kFrags > kMerge ? 2 * kFrags : kMerge) * 64];
-  __shared__ uint8_t seen_s[8][CT * DT][64];  // values that were not finite
+  __shared__ uint8_t seen_s[kWaves][CT * DT][64];  // values that were not finite
   __shared__ int bad_s[2];                    // 1 + the last tile in this buffer with such a V value
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int half = wave >> 2, tid = threadIdx.x & (kHalf - 1);  // waves 0-3: first half of a tile, bring K
+  const int half = wave / kGroups, wc = wave - half * kGroups;  // of a tile; column group
   const int col = lane & 15, grp = lane >> 4;
   const int G = a.H / a.KH, R = a.L * G;
   // Blocks go to the eight dies in turn, the columns with the most keys first. A die would see few of the
@@ -157,12 +173,12 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
   }
   const int z = bx % a.splits, bg = bx / a.splits;
   const int b = bg / a.KH, g = bg - b * a.KH;
-  const int m0 = by * (64 * CT);
+  const int m0 = by * kColumns;
 
   // the block's first and last position
   int hi_p = -1, lo_p = INT32_MAX;
 #pragma unroll
-  for (int i = 0; i < CT; ++i) {
+  for (int i = 0; i < kColumns / 64; ++i) {
     const int p = column_pos(a, b, m0 + 64 * i + lane);
     hi_p = max(hi_p, p);
     lo_p = p < 0 ? lo_p : min(lo_p, p);
@@ -179,27 +195,16 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
   const int t0 = z * per, t1 = min(keys.tiles, t0 + per);
   const long long base = (long long)b * a.kvBatch + (long long)g * D;
 
-  Stage<D, I4> st;
-  // (The two ends differ so that the compiler does not join the branches' last loads into one whose register
-  // is an index, which would put them into memory.)
-  auto load = [&](const Tile& tl) {
-    if (half == 0) {
-      st.load_k(a, base, tl, tid);
-      asm volatile("; K rows");
-    } else {
-      st.load_v(a, base, tl, tid);
-      asm volatile("; V rows");
-    }
-  };
+  Bring st;
   Tile tile = tile_of<kTile>(a, keys, t0 < t1 ? t0 : 0);
-  if (t0 < t1) load(tile);
+  if (t0 < t1) st.load(a, base, tile, threadIdx.x);
   half8_t qh[CT][QT], ql[CT][F32 ? QT : 1];
   float mult[CT], m[CT], l[CT];
   int p[CT];
   float4_t o[CT][DT];
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
-    const int mc = m0 + ((wave & 3) * CT + c) * 16 + col;
+    const int mc = m0 + (wc * CT + c) * 16 + col;
     p[c] = column_pos(a, b, mc);
     Query<D, false, F32> query;
     query.load(a, b, g, mc, p[c] >= 0, grp);
@@ -216,18 +221,15 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
   // tile t + 1's fragments are written while tile t's are used: one barrier per tile
   auto store = [&](int t, const Tile& tl) {
     half8_t* k_s = smem + ((t - t0) & 1) * (kFrags * 64);
-    if (half == 0) {
-      st.store_k(k_s, tid);
-    } else {
-      const half2_t zz = st.store_v(k_s + 4 * QT * 64, tid, !tl.whole);
-      if (!(zz[0] == 0.f && zz[1] == 0.f)) bad_s[(t - t0) & 1] = t + 1;
-    }
+    st.store_k(k_s, threadIdx.x);
+    const half2_t zz = st.store_v(k_s + 4 * QT * 64, threadIdx.x, !tl.whole);
+    if (!(zz[0] == 0.f && zz[1] == 0.f)) bad_s[(t - t0) & 1] = t + 1;
   };
   if (threadIdx.x < 2) bad_s[threadIdx.x] = 0;
   __syncthreads();
   Tile next = tile_of<kTile>(a, keys, t0 + 1 < t1 ? t0 + 1 : t0);
   if (t0 < t1) store(t0, tile);
-  if (t0 + 1 < t1) load(next);
+  if (t0 + 1 < t1) st.load(a, base, next, threadIdx.x);
   __syncthreads();
 
   for (int t = t0; t < t1; ++t) {
@@ -252,7 +254,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
     const Tile after = tile_of<kTile>(a, keys, t + 2 < t1 ? t + 2 : t);
     if (t + 1 < t1) {
       store(t + 1, next);
-      if (t + 2 < t1) load(after);
+      if (t + 2 < t1) st.load(a, base, after, threadIdx.x);
     }
     half8_t ph[CT], pl[CT];
 #pragma unroll
@@ -288,7 +290,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
 #pragma unroll 1
       for (int i = 0; i < DT; ++i) {
         half8_t mark;
-        without_marked(v_s[(i * 2 + half) * 64 + grp * 16 + (col ^ (i & (VD - 1)))], mark);
+        without_marked(v_s[(i * 2 + half) * 64 + grp * 16 + Bring::v_slot(i, col)], mark);
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
           uint8_t* w = &seen_s[wave][c * DT + i][lane];
@@ -306,7 +308,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
-      const half8_t v8 = v_s[(i * 2 + half) * 64 + grp * 16 + (col ^ (i & (VD - 1)))];
+      const half8_t v8 = v_s[(i * 2 + half) * 64 + grp * 16 + Bring::v_slot(i, col)];
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         o[c][i] = mfma(v8, ph[c], o[c][i]);
@@ -326,8 +328,8 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
   }
 
   // the second halves' sums through LDS to the first's
-  float4_t* o_s = reinterpret_cast<float4_t*>(smem) + (wave & 3) * (CT * DT * 64);
-  float2* ml_s = reinterpret_cast<float2*>(reinterpret_cast<float4_t*>(smem) + 4 * CT * DT * 64) + (wave & 3) * (CT * 64);
+  float4_t* o_s = reinterpret_cast<float4_t*>(smem) + wc * (CT * DT * 64);
+  float2* ml_s = reinterpret_cast<float2*>(reinterpret_cast<float4_t*>(smem) + kGroups * CT * DT * 64) + wc * (CT * 64);
   if (half) {
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
