@@ -17,6 +17,8 @@ namespace ns2cache {
 
 using namespace ns2dev;
 
+typedef float float2_t __attribute__((ext_vector_type(2)));
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kGroup = 32;  // values per step and offset of a 4-bit cache
 
@@ -269,18 +271,23 @@ __device__ __forceinline__ float4_t mfma(half4_t a, half4_t b, float4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
 }
 
-// The B operand of the second product: eight weights, rounded to halves, or (F32) as two halves: the leading
-// 11 bits and the rest, which keeps 21 to 22 bits in all.
+// The B operand of the second product: the weights rounded to halves, or (F32) as two halves that keep 22 bits, the
+// second what the first's rounding left (one mixed-precision multiply-add; the factor hides from the compiler, which
+// would make a conversion and a subtraction of it).
 template <bool F32, int N, class H>
 __device__ __forceinline__ void weights(const float (&p)[N], H& hi, H& lo) {
+  float one = 1.f;
+  asm("" : "+s"(one));
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    if constexpr (!F32) {
-      hi[e] = (half_t)p[e];
-    } else {
-      const float lead = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p[e]) & 0xffffe000u);
-      hi[e] = (half_t)lead;
-      lo[e] = (half_t)(p[e] - lead);
+  for (int e = 0; e < N; e += 2) {
+    const half2_t h = __builtin_convertvector(float2_t{p[e], p[e + 1]}, half2_t);
+    hi[e] = h[0];
+    hi[e + 1] = h[1];
+    if constexpr (F32) {
+      const half2_t l = __builtin_convertvector(
+          float2_t{__builtin_fmaf(-(float)h[0], one, p[e]), __builtin_fmaf(-(float)h[1], one, p[e + 1])}, half2_t);
+      lo[e] = l[0];
+      lo[e + 1] = l[1];
     }
   }
 }
