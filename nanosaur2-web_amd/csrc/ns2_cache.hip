@@ -46,7 +46,8 @@ __device__ __forceinline__ float unit8_min(float v) {
 // time: the sum of squares runs over units of 8 lanes (DPP) and then over the head's D / 32 units, the rotation's
 // partner i +- D/2 is D / 8 lanes away, and a 4-bit group is one unit of 8 lanes. Every value is read once and
 // written once, which bounds it; U times as many heads per wave, all asked for at once, keep the memory busy
-// where there are enough of them (8191 tokens x 24 heads of 128 to fp16: 31.5 us with one, 28 with four).
+// where there are enough of them (8191 tokens x 24 heads of 128 to fp16: 30.6 us with one, 29.7, 5.2 TB/s, with
+// four; 2048 tokens 9.0, 9.8). 2400 tokens x 6 heads of 256 to 4 bits 7.4 us.
 template <int D, bool I4, int U>
 __global__ __launch_bounds__(256) void cache_write_kernel(WriteArgs a) {
   constexpr int T = D / 4, HPW = 256 / D;
@@ -226,7 +227,8 @@ Plan plan_of(int batch, int L, int H, int KH, int cap, int window, int sinks) {
   const long long keys = window ? std::min<long long>(cap, (long long)window + sinks + L) : cap;
   Plan p;
   p.prompt = R > kRowsColumns;
-  // enough blocks for the CUs: one each, of few columns two
+  // enough blocks for the CUs: one each, of few columns two (32 single tokens on 16000 4-bit keys: 34.2 us, with one
+  // block each 41.6)
   const long long full = p.prompt ? kCUs : 2 * kCUs;
   const long long heads = std::min((long long)batch * KH, full), tiles = std::min(p.prompt ? (R + 63) / 64 : (R + 15) / 16, full);
   const long long want = full / (heads * tiles);
@@ -279,9 +281,9 @@ int ns2_head_norm_cache(const float* X, int ldx, const int* pos, const float* w_
   NS2_REQUIRE(units <= INT32_MAX, "%s: %lld heads are too many for one launch", fn, units);
   WriteArgs a{X,  pos, w_q, w_k,  cs,   q, k, v, reinterpret_cast<half2_t*>(k_groups), reinterpret_cast<half2_t*>(v_groups), sin_off, kvBatch,
               (unsigned)units, ldx, ldq, ldkv, L, H, KH, cap, rope_rows, q_fmt, eps};
-  // four heads per lane group where that still leaves every SIMD four waves
+  // four heads per lane group where that still leaves every SIMD sixteen waves
   const long long waves = (units + 256 / D - 1) / (256 / D);
-  const bool four = waves >= 4 * 4 * 4 * kCUs;
+  const bool four = waves >= 4 * 16 * 4 * kCUs;
   const unsigned grid = (unsigned)((waves + (four ? 15 : 3)) / (four ? 16 : 4));
   hipStream_t s = ns2::stream();
   ns2::ProfScope prof_("head_norm_cache");

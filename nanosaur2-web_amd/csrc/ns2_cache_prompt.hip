@@ -4,11 +4,19 @@
 // tiles of 64. Its eight waves are four groups of columns (CT tiles of 16 each, queries and accumulators in
 // registers) times two halves of every tile, with a softmax state each; the halves are merged at the end. So
 // every SIMD has two waves to choose from where one block fills a CU, and a wave reads from LDS only its half
-// of a tile. A tile's K and V rows go to LDS once for all waves, as operand fragments, while four waves bring
-// K and four V: K as it lies, V transposed in registers on the way (8 keys x VD dimensions per thread, one byte
-// permutation per pair of values), 4-bit values turned into fp16 there. The next tile's rows are requested
-// before this one's products. Fragments are 1 KB, lane by lane; the 16-byte slots inside one are exchanged
-// (xor) by a pattern of the fragment so that the threads of a row write to different banks.
+// of a tile. A tile's K and V rows go to LDS once for all waves, as operand fragments, every thread bringing the
+// same share of both (the tile ends with the slowest wave): K as it lies, V transposed in registers on the way
+// (4 keys x VD dimensions per thread, one byte permutation per pair of values), 4-bit values turned into fp16
+// there. The next tile's rows are requested before this one's products. Fragments are 1 KB, lane by lane; the
+// 16-byte slots inside one are exchanged (xor) by a pattern of the fragment so that the threads of a row write to
+// different banks.
+//
+// Measured: 2 x 3001 fp32 queries of 16 heads of 128 on 1003 to 4003 4-bit keys of 4 heads 244 us (388 TFLOP/s, and
+// twice that in products, since fp32 takes two), 4096 fp16 queries of 4 heads of 256 in a window of 512 26 us (311
+// TFLOP/s). A tile of the first takes a wave 5400 cycles, of which 2048 keep the matrix cores busy; the rest is
+// mostly VALU work of the two waves of a SIMD (300 instructions each: 4-bit values 115, softmax and weights 130).
+// Heads of 256 are bound by LDS: their 64 columns read each fragment four times (2048 of 4000 cycles). Four waves of
+// 32 columns, which read it twice, leave a SIMD one wave and took 39 us.
 #include "ns2_cache.h"
 
 using namespace ns2cache;
@@ -162,8 +170,9 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
   const int G = a.H / a.KH, R = a.L * G;
   // Blocks go to the eight dies in turn, the columns with the most keys first. A die would see few of the
   // heads then (fewer keys for its cache) but also few of the sequences, which may differ in length: every four
-  // column blocks the sequences move on by one (2 and 3 thousand tokens over a 4-bit cache: 316 us without, 262
-  // with; two equal sequences 365, 374). In a window, where neighbours share keys, each die takes a run of columns.
+  // column blocks the sequences move on by one (8 sequences of 333 to 1000 tokens on a cache of 1003: 168 us
+  // without, 120 with; of equal lengths the same). In a window, where neighbours share keys, each die takes a run of
+  // columns (27.0 us without, 26.0 with, 4096 tokens and heads of 256).
   int by = gridDim.y - 1 - blockIdx.y, bx = (blockIdx.x + blockIdx.y / 4 * (a.KH * a.splits)) % gridDim.x;
   if (a.window) {
     const int n = gridDim.x * gridDim.y, id = blockIdx.x + gridDim.x * blockIdx.y, even = n / 8, odd = n - 8 * even;
@@ -370,7 +379,8 @@ template <int D, bool I4, bool F32>
 void launch(const AttnArgs& a, hipStream_t s) {
   const int R = a.L * (a.H / a.KH);
   const unsigned x = (unsigned)(a.batch * a.KH * a.splits);
-  // two column tiles per wave where that leaves every CU a block (and the registers hold them)
+  // two column tiles per wave where that leaves every CU a block and the registers hold them (2 x 3001 queries of 16
+  // heads of 128: 342 us with one, 244 with two; 1200 queries, 40 blocks x 4 heads: 27, 35)
   if constexpr (D < 256) {
     if ((long long)x * ((R + 127) / 128) >= 256) {
       cache_prompt_kernel<D, I4, F32, 2><<<dim3(x, (R + 127) / 128), kThreads, 0, s>>>(a);

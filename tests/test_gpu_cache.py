@@ -482,10 +482,10 @@ def test_queries_in_place(ns2lib):
 @pytest.mark.parametrize("i4", [False, True])
 @pytest.mark.parametrize("H,KH,D", [(8, 2, 64), (4, 4, 96), (6, 2, 128), (4, 1, 256)])
 def test_long_documents(ns2lib, H, KH, D, i4, fp16):
-    """Thousands of tokens in one call (several heads per lane group) hold what calls of 200 tokens write, bit for bit;
+    """Thousands of tokens in one call (several heads per lane group) hold what calls of 1000 tokens write, bit for bit;
     queries in place too."""
     heads, per = H + 2 * KH, 256 // D
-    L = 16384 * per // (2 * heads) + 77
+    L = 65536 * per // (2 * heads) + 77
     cap = L + 9
     rnd = gen(D)
     x = rnd(2 * L, heads * D)
@@ -495,11 +495,11 @@ def test_long_documents(ns2lib, H, KH, D, i4, fp16):
     got = write(ns2lib, x, pos, H, KH, D, cap, **a)
     seq = x.reshape(2, L, -1)
     want = None
-    for i in range(0, L, 200):
-        part = write(ns2lib, seq[:, i: i + 200].reshape(-1, heads * D).contiguous(), pos[:, i: i + 200].contiguous(), H, KH, D, cap, **a)
+    for i in range(0, L, 1000):
+        part = write(ns2lib, seq[:, i: i + 1000].reshape(-1, heads * D).contiguous(), pos[:, i: i + 1000].contiguous(), H, KH, D, cap, **a)
         if want is None:
             want = {n: t.clone() for n, t in part.items() if n != "q"}
-        n = min(200, L - i)
+        n = min(1000, L - i)
         assert torch.equal(got["q"].reshape(2, L, -1)[:, i: i + n], part["q"].reshape(2, n, -1))
         for b in range(2):
             at = pos[b, i: i + n].long()
