@@ -78,11 +78,14 @@ constexpr int waves() {
   return WK == 16 ? 16 : 4;
 }
 constexpr int kSlabBytes = 48 * 1024;
+// Places of a piece of 8 columns in LDS: an odd number, since threads that write pieces of one row would meet in the
+// same banks otherwise (16 x 4096 x 1536 fp32 8.8 us, so 7.2).
+__host__ __device__ constexpr int places(int rows) { return rows | 1; }
 
 // A block takes 16 rows and, with WK = 1, 64 CT columns (16 CT per wave) over all of K; with WK = 4 or 16, 16 CT
 // columns whose chunks its WK waves take in turn and add up at the end. NR: result registers in use (4 NR rows).
 // SG: 32-column steps per group. The block's rows of x go to LDS a slab of p.slab columns at a time: operand
-// (step, lane group, row), `rows` rows, hi then lo.
+// (step, lane group, row), places(rows) apart, hi then lo.
 template <bool A16, int SG, int NR, int CT, int WK>
 __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p) {
   constexpr int kWaves = waves<WK>();
@@ -128,8 +131,8 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
 
   for (int k0 = 0; k0 < p.K; k0 += p.slab) {
     const int ks = p.K - k0 < p.slab ? p.K - k0 : p.slab;
-    const int n8 = (ks + kChunk - 1) / kChunk * (kChunk / 8), items = rows * n8;  // (zeros behind K, to the end of its chunk)
-    half8_t* lo_s = x_s + items;
+    const int n8 = (ks + kChunk - 1) / kChunk * (kChunk / 8), items = rows * n8, pad = places(rows);  // (zeros behind K, to the end of its chunk)
+    half8_t* lo_s = x_s + pad * n8;
     const int first = k0 / kChunk + (WK == 1 ? 0 : wave), last = (k0 + ks + kChunk - 1) / kChunk;
 #pragma unroll
     for (int s = 0; s < PD; ++s)
@@ -140,7 +143,7 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
         const int r = u / n8, k8 = u - r * n8;
         half8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
         if (8 * k8 < ks) v = *reinterpret_cast<const half8_t*>(static_cast<const half_t*>(p.A) + (long long)(m0 + r) * p.lda + k0 + 8 * k8);
-        x_s[k8 * rows + r] = half8_t{v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
+        x_s[k8 * pad + r] = half8_t{v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
       }
     } else {
       constexpr int NI = (kSlabBytes / 32 + 64 * kWaves - 1) / (64 * kWaves);  // pieces of 8 columns per thread
@@ -183,8 +186,8 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
             hi[e] = (half_t)t;
             lo[e] = (half_t)(t - (float)hi[e]);
           }
-          x_s[k8 * rows + r] = hi;
-          lo_s[k8 * rows + r] = lo;
+          x_s[k8 * pad + r] = hi;
+          lo_s[k8 * pad + r] = lo;
         }
       }
     }
@@ -226,9 +229,9 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
           float4_t d[CT];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const half8_t xh = x_s[(base + 4 * j) * rows + arow];
+            const half8_t xh = x_s[(base + 4 * j) * pad + arow];
             half8_t xl;
-            if constexpr (!A16) xl = lo_s[(base + 4 * j) * rows + arow];
+            if constexpr (!A16) xl = lo_s[(base + 4 * j) * pad + arow];
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
               const half8_t q = codes8(t[c][j]);
@@ -291,11 +294,12 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
 template <bool A16, int SG, int NR, int CT, int WK>
 void launch_rows(I4Args p, hipStream_t s) {
   const int rows = p.M < 16 ? p.M : 16, per = rows * (A16 ? 2 : 4);  // bytes of a column of k
-  p.slab = kSlabBytes / per / kChunk * kChunk;
+  const int padded = places(rows) * (A16 ? 2 : 4);
+  p.slab = std::min(kSlabBytes / per, (kSlabBytes + 4096) / padded) / kChunk * kChunk;  // (three blocks to a CU's LDS)
   if (p.slab > p.K) p.slab = (p.K + kChunk - 1) / kChunk * kChunk;
   constexpr int kWaves = waves<WK>();
   const size_t red = WK > 1 ? sizeof(float) * kWaves * CT * NR * 64 : 0;
-  const size_t lds = std::max<size_t>((size_t)p.slab * per, red);
+  const size_t lds = std::max<size_t>((size_t)p.slab * padded, red);
   const int cols = 16 * CT * (WK == 1 ? kWaves : 1);
   const dim3 grid((unsigned)((p.N + cols - 1LL) / cols), (unsigned)((p.M + 15) / 16));
   linear_i4_kernel<A16, SG, NR, CT, WK><<<grid, 64 * kWaves, lds, s>>>(p);
