@@ -79,7 +79,7 @@ constexpr int waves() {
 }
 constexpr int kSlabBytes = 48 * 1024;
 // Places of a piece of 8 columns in LDS: an odd number, since threads that write pieces of one row would meet in the
-// same banks otherwise (16 x 4096 x 1536 fp32 8.8 us, so 7.2).
+// same banks otherwise (16 x 4096 x 1536 fp32 8.7 us, so 7.2).
 __host__ __device__ constexpr int places(int rows) { return rows | 1; }
 
 // A block takes 16 rows and, with WK = 1, 64 CT columns (16 CT per wave) over all of K; with WK = 4 or 16, 16 CT
@@ -312,13 +312,16 @@ void launch_i4(const I4Args& p, hipStream_t s) {
 }
 
 // By the number of 16 x 16 tiles of the output (us, "a | b": fp16 | fp32 x):
-//  - many tiles: all of K in a wave of 32 columns, loads two chunks ahead (256 x 4096 x 640 10.1 | 12.6,
-//    over four waves 11.7 | 22.3; 12 x 32768 x 2048 16.7 | 19.3, 19.5 | 25.9); with up to four fp16 rows, whose
-//    products cost least, 16 columns and loads four chunks ahead (1 x 262144 x 640 17.6, with 32 columns 19.6);
-//  - few tiles and a K that gives sixteen waves work: over sixteen waves (1 x 8192 x 1536 4.2 | 4.8, over
-//    four 4.6 | 4.9; 16 x 8192 x 1536 5.8 | 9.7, 7.0 | 12.0), of 16 columns up to one block per CU or where rows
-//    cost least (16 x 4096 x 1536 fp32 8.9, with 32 columns 9.6), else of 32 (16 x 8192 x 1536 fp32 9.7, with 16 16.0);
-//  - between: over four waves of 32 columns (8 x 16384 x 4096 fp32 25.5, with 16 columns 35.6; in one wave 30.2).
+//  - many tiles: all of K in a wave of 32 columns, loads two chunks ahead (256 x 4096 x 640 9.9 | 11.2, over four
+//    waves 10.9 | 18.3; 12 x 32768 x 2048 16.7 | 18.7, 18.4 | 24.5); with up to four fp16 rows, whose products cost
+//    least, 16 columns and loads four chunks ahead (1 x 262144 x 640 18.2, with 32 columns 19.9);
+//  - few tiles and a K that gives sixteen waves work: over sixteen waves (1 x 8192 x 1536 4.1 | 4.8, over four 4.6 |
+//    4.9; 16 x 8192 x 1536 5.3 | 8.2, 7.3 | 10.0), of 16 columns up to one block per CU or where rows cost least
+//    (16 x 4096 x 1536 fp32 7.3, with 32 columns 7.9), else of 32 (16 x 8192 x 1536 fp32 8.2, with 16 12.6);
+//  - between: over four waves of 32 columns (8 x 16384 x 4096 fp32 21, with 16 columns 28.6; in one wave 27.8).
+// The bytes bound a table (1 x 262144 x 640: 90 MB at 5.0 TB/s); the smallest calls are a launch and two round trips
+// to memory; many rows are bound by the VALU, which decodes the weights again for every 16 rows (256 x 4096 x 640
+// fp32 120 TFLOP/s; blocks of 32 rows had too few waves and took 15.7).
 template <bool A16, int SG>
 void choose_i4(const I4Args& p, hipStream_t s) {
   const long long tiles = (p.N + 15) / 16 * ((p.M + 15LL) / 16);
