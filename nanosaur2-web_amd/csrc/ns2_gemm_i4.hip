@@ -326,7 +326,7 @@ template <bool A16, int SG>
 void choose_i4(const I4Args& p, hipStream_t s) {
   const long long tiles = (p.N + 15) / 16 * ((p.M + 15LL) / 16);
   const bool light = A16 && p.M <= 4, deep = p.K > 4 * kChunk;
-  if (tiles >= (A16 ? 2048 : 1536)) {
+  if (tiles >= (A16 ? 1792 : 1536)) {
     if constexpr (A16) {
       if (light) return launch_rows<A16, SG, 1, 1, 1>(p, s);
     }

@@ -660,3 +660,94 @@ def test_scales_that_are_not_positive(ns2lib, scale, fp16):
         assert ((got.double() - ref).abs() <= R.attention_bound(ref, vmax, smax.abs(), n, 96, fp16)).all()
         with pytest.raises(ns2.NS2Error, match="scale"):
             attend(ns2lib, cache, q, pos, 50, 3, fp16, scale=math.nan)
+
+
+@pytest.mark.parametrize("i4", [False, True])
+def test_two_streams_at_once(ns2lib, i4):
+    """Calls on two streams, each with work memory of its own, over one cache: the bits of the calls by themselves."""
+    rnd = gen(51)
+    H, KH, D, cap = 8, 2, 128, 5000
+    cache = Cache(rnd, 2, cap, KH, D, i4)
+    calls = []
+    for L, start in ((1, 4900), (6, 3000), (130, 2000)):
+        pos = positions([(start, L), (start // 3, L)], L)
+        q = rnd(2, L, H, D).reshape(2 * L, H * D)
+        need = ns2lib.attention_cache_bytes(2, L, H, KH, D, cap, 0, 0)
+        works = [torch.empty(max(need, 16), dtype=torch.uint8, device=DEV) for _ in range(3)]
+        outs = [torch.zeros(2 * L, H * D, device=DEV) for _ in range(3)]
+        calls.append((L, pos, q, works, outs))
+    streams = [torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def run(i):
+        for L, pos, q, works, outs in calls:
+            ns2lib.attention_cache(q, pos, cache.raw["k"], cache.raw["v"], outs[i], L=L, H=H, ldq=H * D, ldo=H * D, work=works[i],
+                                   **cache.args())
+
+    try:
+        run(0)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for i in (1, 2):
+                ns2lib.set_stream(streams[i].cuda_stream)
+                run(i)
+        torch.cuda.synchronize()
+    finally:
+        ns2lib.set_stream(streams[0].cuda_stream)
+    for _, _, _, _, outs in calls:
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("i4", [False, True])
+def test_recorded_prompts(ns2lib, i4, fp16):
+    """A piece of a prompt and a prompt of many columns recorded together, over work memory of the graph's own: each
+    replay equals eager calls on other work memory, with eager work between the replays."""
+    rnd = gen(52)
+    H, KH, D, cap, dt = 4, 2, 64, 3000, torch.float16 if fp16 else torch.float32
+    cache = Cache(rnd, 1, cap, KH, D, i4)
+    stream = torch.cuda.Stream()
+    ns2lib.set_stream(stream.cuda_stream)
+    try:
+        with torch.cuda.stream(stream):
+            bufs = []
+            for L in (20, 300):
+                pos = torch.zeros(1, L, dtype=torch.int32, device=DEV)
+                q = torch.zeros(L, H * D, dtype=dt, device=DEV)
+                need = ns2lib.attention_cache_bytes(1, L, H, KH, D, cap, 900, 5)
+                bufs.append((L, pos, q, [torch.empty(max(need, 16), dtype=torch.uint8, device=DEV) for _ in range(2)],
+                             [torch.zeros(L, H * D, dtype=dt, device=DEV) for _ in range(2)]))
+
+            def calls(i):
+                for L, pos, q, works, outs in bufs:
+                    ns2lib.attention_cache(q, pos, cache.raw["k"], cache.raw["v"], outs[i], L=L, H=H, ldq=H * D, ldo=H * D, window=900,
+                                           sinks=5, q_fmt=int(fp16), work=works[i], **cache.args())
+
+            stream.synchronize()
+            ns2lib.graph_begin()
+            calls(0)
+            graph = ns2lib.graph_end()
+            for n in range(4):
+                for L, pos, q, _, _ in bufs:
+                    pos.copy_(positions([(600 * n + 7, L - n)], L))
+                    q.copy_(rnd(L, H * D))
+                ns2lib.graph_launch(graph)
+                calls(1)
+                stream.synchronize()
+                for _, _, _, _, outs in bufs:
+                    assert torch.equal(outs[0], outs[1]), f"replay {n}"
+                _ = torch.randn(500, 500, device=DEV).sum().item()
+            ns2lib.graph_destroy(graph)
+    finally:
+        ns2lib.set_stream(torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("i4", [False, True])
+def test_a_cache_of_one_position(ns2lib, i4):
+    """The shortest cache: the one token that fits sees itself, whatever the window."""
+    rnd = gen(53)
+    for H, KH, D in HEADS:
+        cache = Cache(rnd, 2, 1, KH, D, i4)
+        pos = torch.zeros(2, 1, dtype=torch.int32, device=DEV)
+        q = rnd(2, 1, H, D)
+        for window, sinks in ((0, 0), (1, 0), (2**31 - 1, 2**31 - 1)):
+            check(attend(ns2lib, cache, q, pos, window, sinks, False), q, pos, cache, window, sinks, False, f"one {H}/{KH}x{D} i4={i4}")
