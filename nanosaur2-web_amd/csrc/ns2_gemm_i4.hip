@@ -82,20 +82,21 @@ constexpr int kSlabBytes = 48 * 1024;
 // same banks otherwise (16 x 4096 x 1536 fp32 8.7 us, so 7.2).
 __host__ __device__ constexpr int places(int rows) { return rows | 1; }
 
-// A block takes 16 rows and, with WK = 1, 64 CT columns (16 CT per wave) over all of K; with WK = 4 or 16, 16 CT
-// columns whose chunks its WK waves take in turn and add up at the end. NR: result registers in use (4 NR rows).
+// A block takes 16 RT rows and, with WK = 1, 64 CT columns (16 CT per wave) over all of K; with WK = 4 or 16, 16 CT
+// columns whose chunks its WK waves take in turn and add up at the end. NR: result registers in use (4 NR rows of
+// each 16).
 // SG: 32-column steps per group. The block's rows of x go to LDS a slab of p.slab columns at a time: operand
 // (step, lane group, row), places(rows) apart, hi then lo.
-template <bool A16, int SG, int NR, int CT, int WK>
+template <bool A16, int SG, int RT, int NR, int CT, int WK>
 __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p) {
   constexpr int kWaves = waves<WK>();
   extern __shared__ __attribute__((aligned(16))) char smem[];
   half8_t* x_s = reinterpret_cast<half8_t*>(smem);
-  __shared__ uint32_t top_s[16];
+  __shared__ uint32_t top_s[16 * RT];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c16 = lane & 15, g = lane >> 4;
-  const int m0 = blockIdx.y * 16;
-  const int rows = p.M - m0 < 16 ? p.M - m0 : 16;
+  const int m0 = blockIdx.y * (16 * RT);
+  const int rows = p.M - m0 < 16 * RT ? p.M - m0 : 16 * RT;
   const int n0 = (WK == 1 ? blockIdx.x * kWaves + wave : blockIdx.x) * (16 * CT);
   const int kb = p.K / 2, kg = p.K / (32 * SG);
 
@@ -121,13 +122,10 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
     }
   };
 
-  float tot[CT][NR];
+  float tot[RT][CT][NR] = {};
+  int arow[RT];  // this lane's rows of the A operand
 #pragma unroll
-  for (int c = 0; c < CT; ++c)
-#pragma unroll
-    for (int r = 0; r < NR; ++r) tot[c][r] = 0.f;
-
-  const int ar = (c16 >> 2) + 4 * (c16 & 3), arow = ar < rows ? ar : rows - 1;  // this lane's row of the A operand
+  for (int i = 0; i < RT; ++i) arow[i] = min(16 * i + (c16 >> 2) + 4 * (c16 & 3), rows - 1);
 
   for (int k0 = 0; k0 < p.K; k0 += p.slab) {
     const int ks = p.K - k0 < p.slab ? p.K - k0 : p.slab;
@@ -193,11 +191,7 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
     }
     __syncthreads();
 
-    float acc[CT][NR];
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-      for (int r = 0; r < NR; ++r) acc[c][r] = 0.f;
+    float acc[RT][CT][NR] = {};
     for (int chunk = first; chunk < last; chunk += PD * WK) {
 #pragma unroll
       for (int sl = 0; sl < PD; ++sl) {
@@ -226,21 +220,27 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
           for (int c = 0; c < CT; ++c) transpose_rows(t[c]);
           if (ch + PD * WK < last) load(sl, ch + PD * WK);
           const int base = (ch * kChunk - k0) / 8 + g;
-          float4_t d[CT];
+          float4_t d[RT][CT];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const half8_t xh = x_s[(base + 4 * j) * pad + arow];
-            half8_t xl;
-            if constexpr (!A16) xl = lo_s[(base + 4 * j) * pad + arow];
+            half8_t xh[RT], xl[RT];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+              xh[i] = x_s[(base + 4 * j) * pad + arow[i]];
+              if constexpr (!A16) xl[i] = lo_s[(base + 4 * j) * pad + arow[i]];
+            }
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
               const half8_t q = codes8(t[c][j]);
-              if (j % SG == 0) d[c] = float4_t{0.f, 0.f, 0.f, 0.f};
-              d[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, q, d[c], 0, 0, 0);
-              if constexpr (!A16) d[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, q, d[c], 0, 0, 0);
-              if (j % SG == SG - 1) {
 #pragma unroll
-                for (int r = 0; r < NR; ++r) acc[c][r] = fmaf(s[c][j], d[c][r], acc[c][r]);
+              for (int i = 0; i < RT; ++i) {
+                if (j % SG == 0) d[i][c] = float4_t{0.f, 0.f, 0.f, 0.f};
+                d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh[i], q, d[i][c], 0, 0, 0);
+                if constexpr (!A16) d[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl[i], q, d[i][c], 0, 0, 0);
+                if (j % SG == SG - 1) {
+#pragma unroll
+                  for (int r = 0; r < NR; ++r) acc[i][c][r] = fmaf(s[c][j], d[i][c][r], acc[i][c][r]);
+                }
               }
             }
           }
@@ -248,25 +248,25 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
       }
     }
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      float back = 1.f;
-      if constexpr (!A16) {
-        const int row = g + 4 * r;
-        back = ldexpf(1.f, -i4_up(__builtin_bit_cast(float, top_s[row < rows ? row : rows - 1])));
-      }
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-      for (int c = 0; c < CT; ++c) tot[c][r] = fmaf(acc[c][r], back, tot[c][r]);
-    }
+      for (int r = 0; r < NR; ++r) {
+        float back = 1.f;
+        if constexpr (!A16) back = ldexpf(1.f, -i4_up(__builtin_bit_cast(float, top_s[min(16 * i + g + 4 * r, rows - 1)])));
+#pragma unroll
+        for (int c = 0; c < CT; ++c) tot[i][c][r] = fmaf(acc[i][c][r], back, tot[i][c][r]);
+      }
   }
 
   if constexpr (WK > 1) {
     float* red = reinterpret_cast<float*>(smem);  // [wave][c][r][lane]
     constexpr int T = CT * NR;
+    static_assert(RT == 1, "K is split for few rows only");
     __syncthreads();
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
-      for (int r = 0; r < NR; ++r) red[(wave * T + c * NR + r) * 64 + lane] = tot[c][r];
+      for (int r = 0; r < NR; ++r) red[(wave * T + c * NR + r) * 64 + lane] = tot[0][c][r];
     __syncthreads();
     for (int u = wave; u < T; u += kWaves) {
       float sum = 0.f;
@@ -282,53 +282,57 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
       if (n < p.N) {
         const float bi = p.bias ? p.bias[n] : 0.f, gt = p.gate ? p.gate[p.gOff + n] : 1.f;
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          const int m = m0 + g + 4 * r;
-          if (m < m0 + rows) store_i4(p, m, n, tot[c][r], bi, gt);
-        }
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            const int m = m0 + 16 * i + g + 4 * r;
+            if (m < m0 + rows) store_i4(p, m, n, tot[i][c][r], bi, gt);
+          }
       }
     }
   }
 }
 
-template <bool A16, int SG, int NR, int CT, int WK>
+template <bool A16, int SG, int RT, int NR, int CT, int WK>
 void launch_rows(I4Args p, hipStream_t s) {
-  const int rows = p.M < 16 ? p.M : 16, per = rows * (A16 ? 2 : 4);  // bytes of a column of k
-  const int padded = places(rows) * (A16 ? 2 : 4);
-  p.slab = std::min(kSlabBytes / per, (kSlabBytes + 4096) / padded) / kChunk * kChunk;  // (three blocks to a CU's LDS)
+  const int rows = p.M < 16 * RT ? p.M : 16 * RT, size = A16 ? 2 : 4;  // (of a value of x)
+  p.slab = std::min(kSlabBytes / (rows * size), (kSlabBytes + 4096) / (places(rows) * size)) / kChunk * kChunk;  // (three blocks to a CU's LDS)
   if (p.slab > p.K) p.slab = (p.K + kChunk - 1) / kChunk * kChunk;
   constexpr int kWaves = waves<WK>();
   const size_t red = WK > 1 ? sizeof(float) * kWaves * CT * NR * 64 : 0;
-  const size_t lds = std::max<size_t>((size_t)p.slab * padded, red);
+  const size_t lds = std::max<size_t>((size_t)p.slab * places(rows) * size, red);
   const int cols = 16 * CT * (WK == 1 ? kWaves : 1);
-  const dim3 grid((unsigned)((p.N + cols - 1LL) / cols), (unsigned)((p.M + 15) / 16));
-  linear_i4_kernel<A16, SG, NR, CT, WK><<<grid, 64 * kWaves, lds, s>>>(p);
+  const dim3 grid((unsigned)((p.N + cols - 1LL) / cols), (unsigned)((p.M + 16 * RT - 1) / (16 * RT)));
+  linear_i4_kernel<A16, SG, RT, NR, CT, WK><<<grid, 64 * kWaves, lds, s>>>(p);
 }
 template <bool A16, int SG, int CT, int WK>
 void launch_i4(const I4Args& p, hipStream_t s) {
-  if (p.M <= 4) launch_rows<A16, SG, 1, CT, WK>(p, s);
-  else if (p.M <= 8) launch_rows<A16, SG, 2, CT, WK>(p, s);
-  else launch_rows<A16, SG, 4, CT, WK>(p, s);
+  if (p.M <= 4) launch_rows<A16, SG, 1, 1, CT, WK>(p, s);
+  else if (p.M <= 8) launch_rows<A16, SG, 1, 2, CT, WK>(p, s);
+  else launch_rows<A16, SG, 1, 4, CT, WK>(p, s);
 }
 
 // By the number of 16 x 16 tiles of the output (us, "a | b": fp16 | fp32 x):
 //  - many tiles: all of K in a wave of 32 columns, loads two chunks ahead (256 x 4096 x 640 9.9 | 11.2, over four
 //    waves 10.9 | 18.3; 12 x 32768 x 2048 16.7 | 18.7, 18.4 | 24.5); with up to four fp16 rows, whose products cost
-//    least, 16 columns and loads four chunks ahead (1 x 262144 x 640 18.2, with 32 columns 19.9);
+//    least, 16 columns and loads four chunks ahead (1 x 262144 x 640 18.2, with 32 columns 19.9); with many fp16 rows
+//    32 of them per block, unless that leaves an eighth of the blocks' rows empty (32 x 65536 x 2048 34.5, with 16
+//    50; 300 x 27000 x 1536 82, 102; 48 x 65600 x 640 26.9, 24.4. fp32 rows take the same either way, 128 and 131);
 //  - few tiles and a K that gives sixteen waves work: over sixteen waves (1 x 8192 x 1536 4.1 | 4.8, over four 4.6 |
 //    4.9; 16 x 8192 x 1536 5.3 | 8.2, 7.3 | 10.0), of 16 columns up to one block per CU or where rows cost least
 //    (16 x 4096 x 1536 fp32 7.3, with 32 columns 7.9), else of 32 (16 x 8192 x 1536 fp32 8.2, with 16 12.6);
 //  - between: over four waves of 32 columns (8 x 16384 x 4096 fp32 21, with 16 columns 28.6; in one wave 27.8).
 // The bytes bound a table (1 x 262144 x 640: 90 MB at 5.0 TB/s); the smallest calls are a launch and two round trips
-// to memory; many rows are bound by the VALU, which decodes the weights again for every 16 rows (256 x 4096 x 640
-// fp32 120 TFLOP/s; blocks of 32 rows had too few waves and took 15.7).
+// to memory; many rows are bound by the VALU, which decodes the weights again for every block of rows (300 x 27000 x
+// 1536: 300 TFLOP/s, fp32 190).
 template <bool A16, int SG>
 void choose_i4(const I4Args& p, hipStream_t s) {
-  const long long tiles = (p.N + 15) / 16 * ((p.M + 15LL) / 16);
+  const long long high = (p.M + 15LL) / 16, tiles = (p.N + 15) / 16 * high;
   const bool light = A16 && p.M <= 4, deep = p.K > 4 * kChunk;
   if (tiles >= (A16 ? 1792 : 1536)) {
     if constexpr (A16) {
-      if (light) return launch_rows<A16, SG, 1, 1, 1>(p, s);
+      if (light) return launch_rows<A16, SG, 1, 1, 1, 1>(p, s);
+      if (high > 1 && tiles >= 8192 && 8 * high >= 14 * ((high + 1) / 2)) return launch_rows<A16, SG, 2, 4, 2, 1>(p, s);
     }
     launch_i4<A16, SG, 2, 1>(p, s);
   } else if (deep && tiles <= (light ? 512 : 256)) launch_i4<A16, SG, 1, 16>(p, s);

@@ -153,6 +153,7 @@ def test_many_columns(ns2lib):
 @pytest.mark.parametrize("fp16", [False, True])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("M,N,K", [(130, 8200, 384), (33, 30011, 256), (17, 65537, 128), (48, 14003, 1408),  # many rows and columns
+                                   (32, 65540, 256), (61, 33001, 1408), (115, 18003, 640), (300, 8001, 128), (48, 44003, 128),
                                    (1, 65553, 640), (4, 65600, 1152), (6, 65539, 256), (12, 65553, 384), (16, 66000, 128),  # a table
                                    (1, 8181, 640), (7, 8177, 1408), (16, 5003, 640), (40, 2050, 896),  # K over sixteen waves
                                    (1, 20003, 1664), (8, 20003, 640), (16, 10007, 512), (90, 3001, 640)])  # over four
