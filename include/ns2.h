@@ -285,8 +285,8 @@ int ns2_attention_rows_f16kv_oproj(const float* q, const uint16_t* k, const uint
  * for positions below rope_rows, rotated by the table cs at their position (ns2_head_norm's
  * layout; NULL: not rotated). Queries go to q [batch*L, ldq] (q may be X itself), keys and values
  * into the cache at their rows' positions, which have to differ within a sequence. A 4-bit group
- * takes o = half(least value), s = half(range / 15), code = clamp(rint((x - o) / s), 0, 15); a group
- * that holds a NaN or an infinity reads as NaN. The sequences' caches must not overlap.
+ * takes o = half(least value), s = half(range / 15), code = clamp(rint((x - o) / s), 0, 15), with
+ * norm, rotation and codes in 64 bits; a group that holds a NaN or an infinity reads as NaN. The sequences' caches must not overlap.
  *
  * ns2_attention_cache: for each row at position p, head h and g = h / (H / KH),
  *   o[row*ldo + h*D ..] = sum_j softmax_j(scale * <q_row,h, k_j,g>) v_j,g over the keys j <= p with

@@ -36,10 +36,50 @@ __device__ __forceinline__ float unit8_sum(float v) {
   v += dpp<kDppXor2>(v);
   return v + dpp<kDppHalfMirror>(v);
 }
-__device__ __forceinline__ float unit8_min(float v) {
-  v = fminf(v, dpp<kDppXor1>(v));
-  v = fminf(v, dpp<kDppXor2>(v));
-  return fminf(v, dpp<kDppHalfMirror>(v));
+
+// The same in 64 bits.
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint64_t lo = (uint32_t)dpp_i<CTRL>((int)(uint32_t)u), hi = (uint32_t)dpp_i<CTRL>((int)(u >> 32));
+  return __builtin_bit_cast(double, hi << 32 | lo);
+}
+__device__ __forceinline__ double unit8_sum(double v) {
+  v += dpp64<kDppXor1>(v);
+  v += dpp64<kDppXor2>(v);
+  return v + dpp64<kDppHalfMirror>(v);
+}
+__device__ __forceinline__ double unit8_min(double v) {
+  v = fmin(v, dpp64<kDppXor1>(v));
+  v = fmin(v, dpp64<kDppXor2>(v));
+  return fmin(v, dpp64<kDppHalfMirror>(v));
+}
+// Four values of a group of 32 (eight lanes): its step and offset, and their codes, lowest first. A NaN or an
+// infinity makes both NaN.
+__device__ __forceinline__ uint32_t codes_of(const double (&y)[4], half_t& step, half_t& offset) {
+  float bad = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) bad += (float)y[e] - (float)y[e];
+  bad = unit8_sum(bad);
+  const double lo = unit8_min(fmin(fmin(y[0], y[1]), fmin(y[2], y[3])));
+  const double hi = -unit8_min(-fmax(fmax(y[0], y[1]), fmax(y[2], y[3])));
+  step = (half_t)((float)((hi - lo) * (1.0 / 15.0)) + bad);
+  offset = (half_t)((float)lo + bad);
+  const float s = (float)step, inv = s > 0.f ? 1.f / s : 0.f;
+  const double s64 = s, o64 = (double)(float)offset;
+  uint32_t c = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    // the code next to the quotient in 32 bits, moved where the rest says that another is nearer
+    const double d = y[e] - o64;
+    float q = rintf((float)d * inv);
+    const double rest = 2.0 * fma(-(double)q, s64, d);
+    const bool odd = (int)fminf(fmaxf(q, 0.f), 15.f) & 1;
+    if (rest > s64 || (rest == s64 && odd)) q += 1.f;
+    if (rest < -s64 || (rest == -s64 && odd)) q -= 1.f;
+    c |= (uint32_t)(int)(s > 0.f ? fminf(fmaxf(q, 0.f), 15.f) : 0.f) << (4 * e);
+  }
+  return c;
 }
 
 // D / 4 lanes hold one head of one token, four consecutive values each, so that a wave takes 256 / D heads at a
@@ -47,7 +87,11 @@ __device__ __forceinline__ float unit8_min(float v) {
 // partner i +- D/2 is D / 8 lanes away, and a 4-bit group is one unit of 8 lanes. Every value is read once and
 // written once, which bounds it; U times as many heads per wave, all asked for at once, keep the memory busy
 // where there are enough of them (8191 tokens x 24 heads of 128 to fp16: 30.6 us with one, 29.7, 5.2 TB/s, with
-// four; 2048 tokens 9.0, 9.8). 2400 tokens x 6 heads of 256 to 4 bits 7.4 us.
+// four; 2048 tokens 9.0, 9.8).
+//
+// What becomes 4-bit codes is computed in 64 bits, keys from the norm on: a value's last bits in fp32 would decide
+// between two codes, a step of the whole value apart, wherever it lies near their border. 2400 tokens x 6 heads of 256
+// 8.8 us, in fp32 7.4.
 template <int D, bool I4, int U>
 __global__ __launch_bounds__(256) void cache_write_kernel(WriteArgs a) {
   constexpr int T = D / 4, HPW = 256 / D;
@@ -84,32 +128,66 @@ __global__ __launch_bounds__(256) void cache_write_kernel(WriteArgs a) {
   for (int i = 0; i < U; ++i) {
     float x[4] = {xs[i].x, xs[i].y, xs[i].z, xs[i].w};
     const bool is_v = h[i] >= (unsigned)(a.H + a.KH), is_q = h[i] < (unsigned)a.H;
-    const float* w = is_q ? a.w_q : is_v ? nullptr : a.w_k;
-    // (multiply-adds are written out, so that a token's bits do not depend on U)
-    const float ss = unit8_sum(fmaf(x[0], x[0], x[1] * x[1]) + fmaf(x[2], x[2], x[3] * x[3]));
-    float sum = 0.f;
-#pragma unroll
-    for (int n = 0; n < D / 32; ++n) sum += __shfl(ss, (base + 8 * n) & 63);
-    if (w) {
-      const float r = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
-      const float4 w4 = *reinterpret_cast<const float4*>(w + 4 * t);
-      x[0] = x[0] * r * w4.x;
-      x[1] = x[1] * r * w4.y;
-      x[2] = x[2] * r * w4.z;
-      x[3] = x[3] * r * w4.w;
-    }
-    {
-      const int partner = (base + (low ? t + T / 2 : t - T / 2)) & 63;
-      const float c[4] = {cs[i].x, cs[i].y, cs[i].z, cs[i].w}, s[4] = {sn[i].x, sn[i].y, sn[i].z, sn[i].w};
-      float o[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = __shfl(x[e], partner);
-      if (a.cs && !is_v && p[i] >= 0 && p[i] < a.rope_rows) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = fmaf(x[e], c[e], (low ? -o[e] : o[e]) * s[e]);
+    if (!I4 || __builtin_amdgcn_ballot_w64(is_q)) {
+      const float* w = is_q ? a.w_q : is_v ? nullptr : a.w_k;
+      // (multiply-adds are written out, so that a token's bits do not depend on U)
+      const float ss = unit8_sum(fmaf(x[0], x[0], x[1] * x[1]) + fmaf(x[2], x[2], x[3] * x[3]));
+      float sum = 0.f;
+  #pragma unroll
+      for (int n = 0; n < D / 32; ++n) sum += __shfl(ss, (base + 8 * n) & 63);
+      if (w) {
+        const float r = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
+        const float4 w4 = *reinterpret_cast<const float4*>(w + 4 * t);
+        x[0] = x[0] * r * w4.x;
+        x[1] = x[1] * r * w4.y;
+        x[2] = x[2] * r * w4.z;
+        x[3] = x[3] * r * w4.w;
+      }
+      {
+        const int partner = (base + (low ? t + T / 2 : t - T / 2)) & 63;
+        const float c[4] = {cs[i].x, cs[i].y, cs[i].z, cs[i].w}, s[4] = {sn[i].x, sn[i].y, sn[i].z, sn[i].w};
+        float o[4];
+  #pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __shfl(x[e], partner);
+        if (a.cs && !is_v && p[i] >= 0 && p[i] < a.rope_rows) {
+  #pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = fmaf(x[e], c[e], (low ? -o[e] : o[e]) * s[e]);
+        }
       }
     }
     const bool held = lives[i] && p[i] >= 0 && p[i] < a.cap;
+    uint32_t code = 0;
+    half_t step = 0, offset = 0;
+    if constexpr (I4) {
+      // (lanes of queries take part in the exchanges of the others)
+      if (__builtin_amdgcn_ballot_w64(!is_q)) {
+        double y[4] = {xs[i].x, xs[i].y, xs[i].z, xs[i].w};
+        if (a.w_k) {
+          const double s8 = unit8_sum(fma(y[0], y[0], y[1] * y[1]) + fma(y[2], y[2], y[3] * y[3]));
+          double all = 0.0;
+#pragma unroll
+          for (int n = 0; n < D / 32; ++n) all += __shfl(s8, (base + 8 * n) & 63);
+          const float4 w4 = *reinterpret_cast<const float4*>(a.w_k + 4 * t);
+          const double scale = rsqrt(all / D + (double)a.eps);
+          if (!is_v) {
+            y[0] *= scale * w4.x;
+            y[1] *= scale * w4.y;
+            y[2] *= scale * w4.z;
+            y[3] *= scale * w4.w;
+          }
+        }
+        const int partner = (base + (low ? t + T / 2 : t - T / 2)) & 63;
+        const float c[4] = {cs[i].x, cs[i].y, cs[i].z, cs[i].w}, sv[4] = {sn[i].x, sn[i].y, sn[i].z, sn[i].w};
+        double o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __shfl(y[e], partner);
+        if (a.cs && !is_v && p[i] >= 0 && p[i] < a.rope_rows) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = fma(y[e], (double)c[e], (low ? -o[e] : o[e]) * sv[e]);
+        }
+        code = codes_of(y, step, offset);
+      }
+    }
     if (is_q) {
       const long long at = (long long)row[i] * a.ldq + h[i] * D + 4 * t;
       if (held) {
@@ -127,22 +205,9 @@ __global__ __launch_bounds__(256) void cache_write_kernel(WriteArgs a) {
       if (held)
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(cache) + at) = make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
     } else {
-      // offset = the least value, step = range / 15, both rounded to fp16 before the codes are taken;
-      // a NaN or an infinity (x - x is then NaN) makes the group's offset NaN
-      const float bad = unit8_sum(((x[0] - x[0]) + (x[1] - x[1])) + ((x[2] - x[2]) + (x[3] - x[3])));
-      const float lo = unit8_min(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])));
-      const float hi = -unit8_min(-fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-      const half_t sh = (half_t)((hi - lo) / 15.0f), oh = (half_t)(lo + bad);
-      const float s = (float)sh, o = (float)oh;
-      uint32_t c = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float q = s > 0.f ? fminf(fmaxf(rintf((x[e] - o) / s), 0.f), 15.f) : 0.f;
-        c |= (uint32_t)(int)q << (4 * e);
-      }
       if (held) {
-        *reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(cache) + at / 2) = (uint16_t)c;
-        if ((t & 7) == 0) (is_v ? a.vg : a.kg)[at / kGroup] = half2_t{sh, oh};
+        *reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(cache) + at / 2) = (uint16_t)code;
+        if ((t & 7) == 0) (is_v ? a.vg : a.kg)[at / kGroup] = half2_t{step, offset};
       }
     }
   }

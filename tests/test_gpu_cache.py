@@ -444,6 +444,29 @@ def test_four_bit_codes_exactly(ns2lib):
         assert torch.equal(got[n][0].cpu(), codes), n
 
 
+@pytest.mark.parametrize("H,KH,D", HEADS)
+def test_four_bit_keys_exactly(ns2lib, H, KH, D):
+    """Normed and rotated keys, and values: codes and groups are those of 64-bit arithmetic. (Its own error is below
+    2^-45 of a value; one of the 10^5 values here lies as near to a border with a chance below 10^-7.)"""
+    rnd = gen(24 + D)
+    L, cap = 150, 160
+    pos = positions([(5, L), (0, L - 20)], L)
+    x = rnd(2 * L, (H + 2 * KH) * D) * 3
+    w, cs = 1 + 0.1 * rnd(D), R.rope_table(cap, D).to(DEV)
+    got = write(ns2lib, x, pos, H, KH, D, cap, i4=True, fp16=False, wq=w, wk=w, cs=cs, rope_rows=cap, fill=0)
+    flat = pos.flatten()
+    live = flat >= 0
+    heads = x.double().reshape(2 * L, H + 2 * KH, D)
+    b, at = torch.arange(2, device=DEV).repeat_interleave(L)[live], flat[live].long()
+    for n, r in (("k", R.head_norm(heads[:, H: H + KH], w, cs, flat, cap, EPS)), ("v", heads[:, H + KH:])):
+        g = r[live].unflatten(-1, (-1, 32))
+        lo, hi = g.amin(-1), g.amax(-1)
+        step, off = ((hi - lo) / 15).float().half(), lo.float().half()
+        q = ((g - off.double().unsqueeze(-1)) / step.double().unsqueeze(-1)).round().clamp(0, 15)
+        assert torch.equal(got[n + "g"][b, at], torch.stack([step, off], -1)), n
+        assert torch.equal(R.nibbles(got[n][b, at]).double(), q.flatten(-2)), n
+
+
 @pytest.mark.parametrize("i4", [False, True])
 def test_values_that_are_not_numbers(ns2lib, i4):
     """A NaN or an infinity stays visible in its own group (or value) and nowhere else."""
