@@ -77,7 +77,15 @@ template <int WK>
 constexpr int waves() {
   return WK == 16 ? 16 : 4;
 }
-constexpr int kSlabBytes = 48 * 1024;
+// (one block to a CU where sixteen waves run, else three); pieces of 8 columns of fp32 rows that a thread holds.
+template <int WK>
+constexpr int slab_bytes() {
+  return WK == 16 ? 60 * 1024 : 52 * 1024;
+}
+template <int WK>
+constexpr int pieces() {
+  return WK == 16 ? 2 : 6;
+}
 // Places of a piece of 8 columns in LDS: an odd number, since threads that write pieces of one row would meet in the
 // same banks otherwise (16 x 4096 x 1536 fp32 8.7 us, so 7.2).
 __host__ __device__ constexpr int places(int rows) { return rows | 1; }
@@ -144,7 +152,7 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
         x_s[k8 * pad + r] = half8_t{v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
       }
     } else {
-      constexpr int NI = (kSlabBytes / 32 + 64 * kWaves - 1) / (64 * kWaves);  // pieces of 8 columns per thread
+      constexpr int NI = pieces<WK>();
       float4 x[NI][2];
       for (int u = threadIdx.x; u < rows; u += 64 * kWaves) top_s[u] = 0u;
 #pragma unroll
@@ -296,8 +304,11 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
 template <bool A16, int SG, int RT, int NR, int CT, int WK>
 void launch_rows(I4Args p, hipStream_t s) {
   const int rows = p.M < 16 * RT ? p.M : 16 * RT, size = A16 ? 2 : 4;  // (of a value of x)
-  p.slab = std::min(kSlabBytes / (rows * size), (kSlabBytes + 4096) / (places(rows) * size)) / kChunk * kChunk;  // (three blocks to a CU's LDS)
-  if (p.slab > p.K) p.slab = (p.K + kChunk - 1) / kChunk * kChunk;
+  const int room = slab_bytes<WK>() / (places(rows) * size), held = A16 ? room : pieces<WK>() * waves<WK>() * 512 / rows;
+  const int most = std::min(room, held) / kChunk, chunks = (p.K + kChunk - 1) / kChunk;
+  // slabs of about the same number of chunks, if possible as many for each wave
+  const int slabs = (chunks + most - 1) / most, each = (chunks + slabs - 1) / slabs, even = (each + WK - 1) / WK * WK;
+  p.slab = (even <= most && even < chunks ? even : each) * kChunk;
   constexpr int kWaves = waves<WK>();
   const size_t red = WK > 1 ? sizeof(float) * kWaves * CT * NR * 64 : 0;
   const size_t lds = std::max<size_t>((size_t)p.slab * places(rows) * size, red);
