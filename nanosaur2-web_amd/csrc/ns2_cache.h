@@ -239,7 +239,7 @@ struct Query {
 // The reference m of a column trails its maximum by up to 2^kSlack: only a score above m + kSlack moves it
 // and rescales the sums, so that most tiles leave the accumulators alone. Weights are 2^(score - m + kLift),
 // at most 2^(kSlack + kLift): far enough below fp16's largest value, and as far as that allows above its
-// smallest (a weight's rounding is off by 2^-25 at least, 2^-31 of the weight of the reference).
+// smallest (what a weight's two halves leave is off by up to 2^-25, 2^-31 of the weight of the reference).
 constexpr float kSlack = 8.f, kLift = 6.f;
 
 // Scores s[N] (-inf where masked; times mult > 0 they are base-2 logarithms) of the lane's column -> weights in
@@ -271,24 +271,24 @@ __device__ __forceinline__ float4_t mfma(half4_t a, half4_t b, float4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
 }
 
-// The B operand of the second product: the weights rounded to halves, or (F32) as two halves that keep 22 bits, the
-// second what the first's rounding left (one mixed-precision multiply-add; the factor hides from the compiler, which
-// would make a conversion and a subtraction of it).
-template <bool F32, int N, class H>
+// The B operand of the second product: the weights as two halves that keep 22 bits, the second what the first's
+// rounding left (one mixed-precision multiply-add; the factor hides from the compiler, which would make a conversion
+// and a subtraction of it). For fp16 queries too: with one half per weight, the sum of weights that divides the
+// output would have to be one of rounded weights, and the output's error is half as large again as that of its own
+// rounding (2.9e-4 against 2.1e-4).
+template <int N, class H>
 __device__ __forceinline__ void weights(const float (&p)[N], H& hi, H& lo) {
   float one = 1.f;
   asm("" : "+s"(one));
 #pragma unroll
   for (int e = 0; e < N; e += 2) {
     const half2_t h = __builtin_convertvector(float2_t{p[e], p[e + 1]}, half2_t);
+    const half2_t l = __builtin_convertvector(
+        float2_t{__builtin_fmaf(-(float)h[0], one, p[e]), __builtin_fmaf(-(float)h[1], one, p[e + 1])}, half2_t);
     hi[e] = h[0];
     hi[e + 1] = h[1];
-    if constexpr (F32) {
-      const half2_t l = __builtin_convertvector(
-          float2_t{__builtin_fmaf(-(float)h[0], one, p[e]), __builtin_fmaf(-(float)h[1], one, p[e + 1])}, half2_t);
-      lo[e] = l[0];
-      lo[e + 1] = l[1];
-    }
+    lo[e] = l[0];
+    lo[e + 1] = l[1];
   }
 }
 

@@ -11,9 +11,9 @@
 // 16-byte slots inside one are exchanged (xor) by a pattern of the fragment so that the threads of a row write to
 // different banks.
 //
-// Measured: 2 x 3001 fp32 queries of 16 heads of 128 on 1003 to 4003 4-bit keys of 4 heads 244 us (388 TFLOP/s, and
-// twice that in products, since fp32 takes two), 4096 fp16 queries of 4 heads of 256 in a window of 512 26 us (311
-// TFLOP/s). A tile of the first takes a wave about 5100 cycles, of which 2048 keep the matrix cores busy; the rest is
+// Measured: 2 x 3001 fp32 queries of 16 heads of 128 on 1003 to 4003 4-bit keys of 4 heads 248 us (382 TFLOP/s, and
+// twice that in products, since fp32 takes two), 4096 fp16 queries of 4 heads of 256 in a window of 512 28 us (290
+// TFLOP/s, and half as much again in products: the weights take two). A tile of the first takes a wave about 5100 cycles, of which 2048 keep the matrix cores busy; the rest is
 // mostly VALU work of the two waves of a SIMD (300 instructions each: 4-bit values 115, softmax and weights 130).
 // Heads of 256 are bound by LDS: their 64 columns read each fragment four times (2048 of 4000 cycles). Four waves of
 // 32 columns, which read it twice, leave a SIMD one wave and took 39 us.
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[c][i] *= corr;
       }
-      weights<F32>(w, ph[c], pl[c]);
+      weights(w, ph[c], pl[c]);
     }
     if (!tile.whole && bad_s[(t - t0) & 1] == t + 1) {  // (for all waves)
       half8_t vis[CT];
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(kThreads, 2) void cache_prompt_kernel(AttnArgs a) {
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         o[c][i] = mfma(v8, ph[c], o[c][i]);
-        if constexpr (F32) o[c][i] = mfma(v8, pl[c], o[c][i]);
+        o[c][i] = mfma(v8, pl[c], o[c][i]);
       }
     }
     tile = next;

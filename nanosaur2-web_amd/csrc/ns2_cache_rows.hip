@@ -9,7 +9,7 @@
 //
 // Measured, with the join of the splits: 16 fp16 tokens of 16 heads on 16384 fp16 keys of 4 heads of 128 98 us (the
 // cache at 5.5 TB/s, a copy reads and writes 5.2); 32 tokens of 4 heads on up to 16000 4-bit keys of one head of 256
-// 34 us (3.2 TB/s: eight 4-bit values of a lane take 13 instructions, the VALU is busy 60 % of the time); one fp32
+// 38 us (2.9 TB/s: eight 4-bit values of a lane take 13 instructions, the VALU is busy 60 % of the time); one fp32
 // token on a window of 516 fp16 keys of 256 10.4 us, the chain of two launches (position, keys, merge; sums, output).
 #include "ns2_cache.h"
 
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) 
       for (int i = 0; i < DT; ++i) o[i] *= corr;
     }
     Part ph, pl;
-    weights<F32>(s, ph, pl);
+    weights(s, ph, pl);
     bool apart = false;
     if (!tile.whole) {
       half2_t zz = {0.f, 0.f};
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) 
     if (!apart) {
       vx.each([&](int i, Part v) {
         o[i] = mfma(v, ph, o[i]);
-        if constexpr (F32) o[i] = mfma(v, pl, o[i]);
+        o[i] = mfma(v, pl, o[i]);
       });
     } else {
       Part vis;
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache_rows_kernel(AttnArgs a) 
         Part mark;
         v = without_marked(v, mark);
         o[i] = mfma(v, ph, o[i]);
-        if constexpr (F32) o[i] = mfma(v, pl, o[i]);
+        o[i] = mfma(v, pl, o[i]);
         seen_s[wave][i][lane] |= seen_bits(mfma(mark, vis, float4_t{0.f, 0.f, 0.f, 0.f}));
         __builtin_amdgcn_sched_barrier(0);
       });

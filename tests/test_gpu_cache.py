@@ -774,3 +774,46 @@ def test_a_cache_of_one_position(ns2lib, i4):
         q = rnd(2, 1, H, D)
         for window, sinks in ((0, 0), (1, 0), (2**31 - 1, 2**31 - 1)):
             check(attend(ns2lib, cache, q, pos, window, sinks, False), q, pos, cache, window, sinks, False, f"one {H}/{KH}x{D} i4={i4}")
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("L", [1, 5, 70, 300])
+def test_values_that_are_all_alike(ns2lib, L, D, i4, fp16):
+    """Where every visible key holds the same values, the output is these values, however the weights lie: some keys at
+    the maximum and hundreds below it that share a score, so that roundings of their weight do not average out. Weights
+    taken in 22 bits and two sums over n <= 1001 keys in fp32 leave 2^-21 + 2 n 2^-24 < 1.3e-4 of a value; an fp16
+    output is then the value itself (its neighbours' borders are 2^-12 = 2.4e-4 away), also at fp16's largest."""
+    cap, H, KH = 1001, 8, 2
+    cache = Cache(gen(61), 1, cap, KH, D, i4)
+    v = torch.linspace(-3, 3, D, device=DEV).half()
+    v[::32], v[5::32] = 65504.0, -65504.0
+    if i4:
+        # one step of 0 per group: the group's value is its offset
+        v = v[::32].repeat_interleave(32) * torch.where(torch.arange(D, device=DEV) % 64 < 32, 1.0, -1.0).half()
+        cache.raw["v"].zero_()
+        cache.group_view("v")[..., 0], cache.group_view("v")[..., 1] = 0.0, v[::32]
+    else:
+        cache.view(cache.raw["v"], 1).copy_(v)
+    pos = positions([(cap - L, L)], L)
+    q = torch.zeros(1, L, H, D, device=DEV)
+    q[..., 3] = 1.0
+    k = torch.zeros(1, cap, KH, D, device=DEV)
+    k[0, :, :, 3] = -1.0
+    k[0, ::16] = 0.0  # (in every tile, so that no part of the keys has the lower score as its own maximum)
+    if i4:
+        codes, groups = R.cache_codes(k)
+        cache.view(cache.raw["k"], 2).copy_(codes)
+        cache.group_view("k").copy_(groups)
+    else:
+        cache.view(cache.raw["k"], 1).copy_(k.half())
+    # weights of the many about half way between two halves, just above or below, where one rounding is off most
+    for m in (1 + 20.47 / 1024, 1 + 20.53 / 1024, 1 + 0.53 / 1024, 1.5 + 0.47 / 1024, 1.25 + 0.53 / 1024):
+        score = -math.log(2) + math.log(m)
+        got = attend(ns2lib, cache, q, pos, 0, 0, fp16, scale=-score)
+        if fp16:
+            assert torch.equal(got, v.expand_as(got)), f"weight {m}"
+        else:
+            # (and the output's own rounding)
+            assert ((got.double() - v.double()).abs() <= v.double().abs() * (2.0**-21 + 2 * cap * 2.0**-24 + 2.0**-22)).all(), f"weight {m}"
