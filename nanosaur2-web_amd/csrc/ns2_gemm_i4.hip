@@ -25,10 +25,10 @@ struct I4Args {
   int slab;  // columns of k whose rows of x are in LDS at a time
 };
 
-// The power of two that takes a row's largest magnitude to below 2^14.
+// The power of two that takes a row's largest finite magnitude to below 2^14.
 __device__ __forceinline__ int i4_up(float top) {
   const int up = 14 - __builtin_amdgcn_frexp_expf(top);
-  return top > 0.f && top < INFINITY ? (up < 120 ? up : 120) : 0;
+  return top > 0.f ? (up < 120 ? up : 120) : 0;
 }
 
 // Epilogue of one output element, as every linear's (gemm.js:159-164).
@@ -166,13 +166,22 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
         }
       }
       __syncthreads();
-      // magnitudes order as their bits do; four neighbours share a row (n8 is a multiple of 4)
+      // magnitudes order as their bits do; four neighbours share a row (n8 is a multiple of 4). What is finite decides
+      // the scaling.
+      uint32_t infinite = 0;  // pieces that hold an infinity
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int u = threadIdx.x + 64 * kWaves * i;
         const float4 a = x[i][0], b = x[i][1];
         float top = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
                           fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
+        if (top == INFINITY) {
+          infinite |= 1u << i;
+          const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+          top = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
+        }
         top = fmaxf(top, dpp<kDppXor1>(top));
         top = fmaxf(top, dpp<kDppXor2>(top));
         if (u < items && (threadIdx.x & 3) == 0) atomicMax(&top_s[u / n8], __builtin_bit_cast(uint32_t, top));
@@ -191,6 +200,10 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
             const float t = ldexpf(v[e], up);
             hi[e] = (half_t)t;
             lo[e] = (half_t)(t - (float)hi[e]);
+          }
+          if (infinite >> i & 1) {  // an infinity is all in hi
+#pragma unroll
+            for (int e = 0; e < 8; ++e) lo[e] = fabsf(v[e]) == INFINITY ? (half_t)0.f : lo[e];
           }
           x_s[k8 * pad + r] = hi;
           lo_s[k8 * pad + r] = lo;

@@ -227,3 +227,37 @@ def test_refusals(ns2lib, change):
     if "group" in change or change.get("K") == 80:
         with pytest.raises(ns2.NS2Error, match="ns2_quantize_i4"):
             ns2lib.quantize_i4(t["A"], t["W"], t["scale"], 32, a["K"], a["group"])
+
+
+def infinite_classes(x, W):
+    """0 where an output of x W^T is finite, 1 and -1 where it is an infinity, 2 where it is NaN, in 64 bits."""
+    y = x.double() @ W.t()
+    return torch.where(torch.isnan(y), 2, torch.where(torch.isinf(y), y.sign(), 0.0))
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 256), (7, 40, 96), (16, 1030, 2080), (33, 30011, 256), (1, 66000, 640), (12, 66000, 128),
+                                   (9, 20003, 1664), (40, 2050, 896), (20, 1040, 6144)])
+def test_infinite_activations(ns2lib, M, N, K, fp16):
+    """An infinity in a row of A makes each of the row's outputs the infinity that its weight's sign says, NaN where the
+    weight is 0 or where two infinities meet with other signs; what is finite beside it decides nothing. Other rows are
+    those of a call without it."""
+    g, rnd = gen(M + N + K)
+    codes, scale = weight(g, N, K, 32)
+    W = R.i4_weight(codes, scale, 32)
+    x = rnd(M, K)
+    clean, _, _ = run(ns2lib, x, codes, scale, 32, fp16=fp16, K=K)
+    y = x.clone()
+    bad = torch.zeros(M, dtype=torch.bool, device=DEV)
+    for r, put in ((0, {K // 3: math.inf}), (M // 2, {K - 1: -math.inf}), (M - 1, {1: math.inf, K // 2: -math.inf})):
+        if bad[r]:
+            continue
+        bad[r] = True
+        for k, v in put.items():
+            y[r, k] = v
+    if not fp16:
+        y[0, K // 2 + 1] = 1e30  # (finite: beyond fp16's range)
+    got, _, _ = run(ns2lib, y, codes, scale, 32, fp16=fp16, K=K)
+    kinds = torch.where(torch.isnan(got), 2, torch.where(torch.isinf(got), got.sign(), 0.0)).double()
+    assert torch.equal(kinds, infinite_classes(y, W))
+    assert torch.equal(got[~bad], clean[~bad])
