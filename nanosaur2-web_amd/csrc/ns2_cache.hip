@@ -303,6 +303,16 @@ Plan plan_of(int batch, int L, int H, int KH, int cap, int window, int sinks) {
   return p;
 }
 
+// Whether rows of x (wx bytes, ldx bytes apart) and of y share a byte. Rows that lie between each other's, at one
+// distance, do not; at different distances, ranges that meet count as sharing.
+bool rows_meet(const void* x, long long ldx, long long wx, const void* y, long long ldy, long long wy, long long rows) {
+  const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
+  if (a + (uintptr_t)((rows - 1) * ldx + wx) <= b || b + (uintptr_t)((rows - 1) * ldy + wy) <= a) return false;
+  if (ldx != ldy) return true;
+  const long long from = (long long)(b >= a ? (b - a) % ldx : (ldx - (a - b) % ldx) % ldx);  // y's row within x's
+  return from < wx || from + wy > ldx;
+}
+
 // The argument checks that both entry points share.
 int check_cache(const char* fn, const void* q, const int* pos, const void* k, const void* v, const void* kg, const void* vg,
                 int batch, int L, int H, int KH, int D, int ldq, int cap, int ldkv, long long kvBatch, int q_fmt) {
@@ -338,6 +348,10 @@ int ns2_head_norm_cache(const float* X, int ldx, const int* pos, const float* w_
   NS2_REQUIRE(X && aligned(X, 16) && ldx % 4 == 0 && ldx >= (H + 2LL * KH) * D,
               "%s: X must hold 16-byte aligned rows of (H + 2 KH) * D values (ldx=%d)", fn, ldx);
   NS2_REQUIRE(aligned(w_q, 16) && aligned(w_k, 16), "%s: the norm weights must be 16-byte aligned", fn);
+  // (in place a lane overwrites what it has read itself, and nothing else, only in rows of the same type and distance)
+  const long long rows = (long long)batch * L, wx = 4 * (H + 2LL * KH) * D, wq = (q_fmt ? 2LL : 4LL) * H * D;
+  NS2_REQUIRE((q == X && !q_fmt && ldq == ldx) || !rows_meet(X, 4LL * ldx, wx, q, (q_fmt ? 2LL : 4LL) * ldq, wq, rows),
+              "%s: q overlaps X (q may be X itself as fp32 with ldq == ldx)", fn);
   if (cs)
     NS2_REQUIRE(aligned(cs, 16) && sin_off % 4 == 0 && rope_rows >= 0 && sin_off >= 0, "%s: the rotation table must be 16-byte aligned",
                 fn);

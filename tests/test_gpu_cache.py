@@ -817,3 +817,55 @@ def test_values_that_are_all_alike(ns2lib, L, D, i4, fp16):
         else:
             # (and the output's own rounding)
             assert ((got.double() - v.double()).abs() <= v.double().abs() * (2.0**-21 + 2 * cap * 2.0**-24 + 2.0**-22)).all(), f"weight {m}"
+
+
+def test_queries_over_other_rows_are_refused(ns2lib):
+    """q may be X itself only where a lane overwrites no more than what it has read: fp32 at X's distance. Any other rows
+    that share bytes with X's would be written before other blocks have read them."""
+    import ns2
+
+    H, KH, D, L = 4, 2, 64, 3
+    width = (H + 2 * KH) * D
+    x = torch.arange(4 * L * width, device=DEV, dtype=torch.float32)
+    before = x.clone()
+    k, v = (torch.zeros(L, KH * D, dtype=torch.float16, device=DEV) for _ in "kv")
+    pos = positions([(0, L)], L)
+    a = dict(batch=1, L=L, H=H, KH=KH, D=D, cap=L, ldkv=KH * D, kvBatch=L * KH * D)
+    at = x.data_ptr() + 4 * L * width
+    for off, ldq, q_fmt in ((0, width, 1), (0, 2 * width, 1), (0, H * D, 0), (0, width + 4, 0), (4 * D, width, 0), (-4 * D, width, 0),
+                            (4 * width, width, 0), (-4 * width, width, 0), (4 * (width - D), width, 0), (4 * (H * D - 4), width, 0),
+                            (4 * L * width - 16, H * D, 0), (-16, H * D, 1), (16 - 4 * H * D * L, H * D, 0)):
+        with pytest.raises(ns2.NS2Error, match="q overlaps X"):
+            ns2lib.head_norm_cache(at, pos, at + off, k, v, ldx=width, ldq=ldq, q_fmt=q_fmt, **a)
+    torch.cuda.synchronize()
+    assert torch.equal(x, before) and (k == 0).all() and (v == 0).all()
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+def test_queries_beside_the_rows(ns2lib, fp16):
+    """Rows of q between the rows of X in one buffer, right behind them and right before them, hold what rows of their own
+    hold; X stays."""
+    rnd = gen(62)
+    H, KH, D, L = 4, 1, 96, 33
+    width, per = (H + 2 * KH) * D, H * D // (2 if fp16 else 1)  # (floats of a row of q)
+    w, cs, pos = 1 + 0.1 * rnd(D), R.rope_table(L, D).to(DEV), positions([(0, L)], L)
+    data = rnd(L, width)
+    dt = torch.float16 if fp16 else torch.float32
+    a = dict(batch=1, L=L, H=H, KH=KH, D=D, cap=L, ldkv=KH * D, kvBatch=L * KH * D, w_q=w, w_k=w, cs=cs, sin_off=cs.numel() // 2,
+             rope_rows=L, q_fmt=int(fp16))
+
+    def caches():
+        return [torch.zeros(L, KH * D, dtype=torch.float16, device=DEV) for _ in "kv"]
+
+    own, want = torch.zeros(L, H * D, dtype=dt, device=DEV), caches()
+    ns2lib.head_norm_cache(data, pos, own, *want, ldx=width, ldq=H * D, **a)
+    for x0, q0, ld in ((0, width, width + per), (per, 0, width + per), (0, width + 8, width + per + 8), (0, L * width, 0), (L * per, 0, 0)):
+        buf = torch.full((L * (width + per + 8),), 3.0, device=DEV)
+        ldx, ldq = ld or width, ld or per
+        x = torch.as_strided(buf, (L, width), (ldx, 1), x0)
+        x.copy_(data)
+        got = caches()
+        ns2lib.head_norm_cache(buf.data_ptr() + 4 * x0, pos, buf.data_ptr() + 4 * q0, *got, ldx=ldx, ldq=ldq * (2 if fp16 else 1), **a)
+        torch.cuda.synchronize()
+        q = torch.as_strided(buf, (L, per), (ldq, 1), q0).contiguous().view(dt)
+        assert torch.equal(q, own) and torch.equal(x, data) and all(torch.equal(m, n) for m, n in zip(got, want))
