@@ -191,7 +191,7 @@ int ns2_tile_bf16_weight(const uint16_t* W, uint16_t* Wt, int N, int K);
  * that the codes stand for. (The parts are taken after scaling by a power of two per row: a value
  * below 2^-16 of its row's largest keeps fewer bits, none below 2^-39 of it.) Made for the few rows
  * of single tokens and conditioning vectors; any M runs. Rows of A and W 16-byte aligned, M at most
- * 2^20 - 16, N 2^29. No counterpart in the reference. */
+ * 2^20 - 16, N 2^29, K 2^30. No counterpart in the reference. */
 int ns2_linear_i4(const void* A, int a_fmt, int lda, const uint8_t* W, const uint16_t* scale,
                   const float* bias, const float* add, float* C, int M, int N, int K, int group,
                   int ldc, long long cOff, float alpha, int act, int resid, const float* gate,

@@ -431,7 +431,7 @@ int ns2_linear_i4(const void* A, int a_fmt, int lda, const uint8_t* W, const uin
   NS2_REQUIRE(act >= NS2_ACT_NONE && act <= NS2_ACT_GELU_TANH, "%s: unknown activation %d", fn, act);
   NS2_REQUIRE(aligned(A, 16) && lda % (a_fmt ? 8 : 4) == 0 && aligned(W, 16) && aligned(scale, 2),
               "%s: the rows of A and W must be 16-byte aligned (lda a multiple of %d)", fn, a_fmt ? 8 : 4);
-  NS2_REQUIRE(M <= 16LL * 65535 && N <= 1 << 29, "%s: M=%d, N=%d are too many for one launch", fn, M, N);
+  NS2_REQUIRE(M <= 16LL * 65535 && N <= 1 << 29 && K <= 1 << 30, "%s: M=%d, N=%d, K=%d are too many for one launch", fn, M, N, K);
   I4Args p{A,  W,   reinterpret_cast<const half_t*>(scale), bias, add, C, gate, cOff, gOff, lda, ldc, M, N, K, group, alpha,
            act, resid};
   ns2::ProfScope prof_("linear_i4");

@@ -261,3 +261,36 @@ def test_infinite_activations(ns2lib, M, N, K, fp16):
     kinds = torch.where(torch.isnan(got), 2, torch.where(torch.isinf(got), got.sign(), 0.0)).double()
     assert torch.equal(kinds, infinite_classes(y, W))
     assert torch.equal(got[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("a_fmt", [0, 1])
+def test_widths_near_the_end_of_32_bits_are_refused(ns2lib, a_fmt):
+    """K's last chunk of 128 columns would end past 2^31; refused before any launch."""
+    import ns2
+
+    C = torch.zeros(64, device=DEV)
+    p = C.data_ptr()
+    for K, group in (((1 << 31) - 32, 32), ((1 << 31) - 128, 128), ((1 << 30) + 32, 32)):
+        with pytest.raises(ns2.NS2Error, match="ns2_linear_i4"):
+            ns2lib.call("ns2_linear_i4", p, a_fmt, K, p, p, None, None, p, 1, 1, K, group, 1, 0, 1.0, 0, 0, None, 0)
+    torch.cuda.synchronize()
+    assert (C == 0).all()
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+def test_a_wide_row(ns2lib, fp16):
+    """K of millions: small whole numbers at a few places, the first and the last columns among them, whose sums are exact."""
+    g, rnd = gen(9)
+    K = 1 << 22
+    for M, N in ((1, 3), (5, 17)):
+        codes = torch.randint(0, 256, (N, K // 2), generator=g, device=DEV, dtype=torch.uint8)
+        scale = torch.full((N, K // 128), 0.5, dtype=torch.float16, device=DEV)
+        x = torch.zeros(M, K, device=DEV)
+        at = torch.cat([torch.randint(0, K, (500,), generator=g, device=DEV), torch.tensor([0, 127, 128, K - 129, K - 128, K - 1], device=DEV)])
+        x[:, at] = torch.randint(-8, 9, (M, len(at)), generator=g, device=DEV).float()
+        C = torch.empty(M, N, device=DEV)
+        ns2lib.linear_i4(x.half() if fp16 else x, int(fp16), K, codes, scale, C, M, N, K, 128)
+        cols = torch.unique(at)
+        byte = codes[:, cols // 2].long()
+        w = torch.where(cols % 2 == 1, byte >> 4, byte & 15).double() - 8
+        assert torch.equal(C.double(), x[:, cols].double() @ w.t() * 0.5)
