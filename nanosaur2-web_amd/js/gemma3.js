@@ -207,24 +207,35 @@ export class Gemma3 {
     const layers = this.layers.map(() => ops.kvCache(this.gpu, { batch, capacity, KH, D, bits }));
     return {
       batch, capacity, bits, sinks, layers, lengths: new Array(batch).fill(0), cs: this.ropeTables(capacity),
+      last: Promise.resolve(), // never rejects; settles when every extend so far has
       destroy: () => layers.forEach((c) => c.destroy()),
     };
   }
 
   // The next tokens of a cache's sequences: ids is one array of token ids per sequence (or, for a batch of one, the
   // array itself), of unequal lengths if need be. Returns the normed hidden states [batch * L, 640], L the longest
-  // array's length; rows b * L + i past a sequence's own tokens hold nothing.
-  async extend(cache, ids) {
-    const lists = cache.batch === 1 && !Array.isArray(ids[0]) ? [ids] : ids;
-    const { pos, L } = this.positions(cache, lists.map((t) => t.length));
-    const padded = [];
-    for (const t of lists) for (let i = 0; i < L; i++) padded.push(i < t.length ? t[i] : t.length ? t[0] : 0);
-    const rows = await this.st.rows("model.embed_tokens.weight", padded);
-    const posT = this.gpu.fromArray(pos, [pos.length]);
-    const y = this.extendEmbedded(cache, this.embed(rows, padded.length), posT, L);
-    posT.release();
-    lists.forEach((t, b) => { cache.lengths[b] += t.length; });
-    return y;
+  // array's length; rows b * L + i past a sequence's own tokens hold nothing. Calls on one cache take effect in the
+  // order in which they were made, also where none waits for the one before; one that fails adds no token.
+  extend(cache, ids) {
+    const run = async (before) => {
+      const lists = cache.batch === 1 && !Array.isArray(ids[0]) ? [ids] : ids;
+      const counts = lists.map((t) => t.length);
+      const L = Math.max(0, ...counts);
+      const padded = [];
+      for (const t of lists) for (let i = 0; i < L; i++) padded.push(i < t.length ? t[i] : t.length ? t[0] : 0);
+      const [rows] = await Promise.all([this.st.rows("model.embed_tokens.weight", padded), before]);
+      // from here on nothing waits: no other call and no recorded step comes between the positions and the lengths
+      const { pos } = this.positions(cache, counts);
+      const posT = this.gpu.fromArray(pos, [pos.length]);
+      const y = this.extendEmbedded(cache, this.embed(rows, padded.length), posT, L);
+      posT.release();
+      counts.forEach((n, b) => { cache.lengths[b] += n; });
+      return y;
+    };
+    const before = cache.last;
+    const done = run(before);
+    cache.last = done.catch(() => before);
+    return done;
   }
 
   // Positions of the next counts[b] tokens of each sequence, -1 for padding up to the longest.

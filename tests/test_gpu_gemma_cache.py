@@ -8,6 +8,7 @@ most 5e-2 after 17 layers that add up at random."""
 
 import json
 import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -161,3 +162,14 @@ def test_chain_of_calls(ns2lib, i4cache):
         od = o.double()
         slack = (H * D + 4) * 2.0**-24 * (od.abs() @ ws["o"][2].abs().t())
         assert ((y.double() - od @ ws["o"][2].t()).abs() <= slack).all()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_calls_in_flight_and_steps_of_one_sequence(model, bits):
+    """Two sequences: calls that do not wait for each other give the bits of calls one by one, and a recorded step that
+    one sequence sits out those of an eager call."""
+    script = os.path.join(os.path.dirname(os.path.abspath(__file__)), "js", "extend_overlap.mjs")
+    p = subprocess.run(["node", script, model[1], str(bits)], capture_output=True, text=True, timeout=110)
+    assert p.returncode == 0, p.stderr[-2000:]
+    got = json.loads(p.stdout.strip().splitlines()[-1])
+    assert got == {"overlap": 0, "recorded": 0, "lengths": [[6, 6], [6, 6], [9, 9], [9, 9]]}
