@@ -227,8 +227,12 @@ export class Gemma3 {
       // from here on nothing waits: no other call and no recorded step comes between the positions and the lengths
       const { pos } = this.positions(cache, counts);
       const posT = this.gpu.fromArray(pos, [pos.length]);
-      const y = this.extendEmbedded(cache, this.embed(rows, padded.length), posT, L);
-      posT.release();
+      let y;
+      try {
+        y = this.extendEmbedded(cache, this.embed(rows, padded.length), posT, L);
+      } finally {
+        posT.release();
+      }
       counts.forEach((n, b) => { cache.lengths[b] += n; });
       return y;
     };
@@ -258,25 +262,33 @@ export class Gemma3 {
     const gpu = this.gpu;
     const { hidden, heads: H } = GEMMA;
     const [csLocal, csGlobal] = cache.cs;
-    let h = ops.rmsnorm(gpu, x, this.layers[0].inNorm, hidden);
-    this.layers.forEach((l, i) => {
-      const kv = cache.layers[i];
-      const qkv = ops.linear(gpu, h, l.qkv, { name: "te.qkv" });
-      h.release();
-      const q = ops.headNormCache(gpu, qkv, pos, kv, { L, H, wq: l.qn, wk: l.kn, cs: l.global ? csGlobal : csLocal,
-        half: l.o.kind === "i4" });
-      qkv.release();
-      const a = ops.attentionCache(gpu, q, pos, kv, { L, H, window: l.global ? 0 : GEMMA.window, sinks: cache.sinks });
-      q.release();
-      const h2 = ops.linearAddRmsnorm(gpu, a, l.o, x, l.postAttnNorm, l.preMlpNorm);
-      a.release();
-      const g = ops.linearGlu(gpu, h2, l.gateUp, "gelu_tanh");
-      h2.release();
-      h = ops.linearAddRmsnorm(gpu, g, l.down, x, l.postMlpNorm, i + 1 < this.layers.length ? this.layers[i + 1].inNorm : this.norm);
-      g.release();
-    });
-    x.release();
-    return h;
+    const held = new Set([x]); // what goes back to the pool if an op throws
+    const hold = (t) => { held.add(t); return t; };
+    const drop = (t) => { held.delete(t); t.release(); };
+    try {
+      let h = hold(ops.rmsnorm(gpu, x, this.layers[0].inNorm, hidden));
+      this.layers.forEach((l, i) => {
+        const kv = cache.layers[i];
+        const qkv = hold(ops.linear(gpu, h, l.qkv, { name: "te.qkv" }));
+        drop(h);
+        const q = hold(ops.headNormCache(gpu, qkv, pos, kv, { L, H, wq: l.qn, wk: l.kn, cs: l.global ? csGlobal : csLocal,
+          half: l.o.kind === "i4" }));
+        drop(qkv);
+        const a = hold(ops.attentionCache(gpu, q, pos, kv, { L, H, window: l.global ? 0 : GEMMA.window, sinks: cache.sinks }));
+        drop(q);
+        const h2 = hold(ops.linearAddRmsnorm(gpu, a, l.o, x, l.postAttnNorm, l.preMlpNorm));
+        drop(a);
+        const g = hold(ops.linearGlu(gpu, h2, l.gateUp, "gelu_tanh"));
+        drop(h2);
+        const next = i + 1 < this.layers.length ? this.layers[i + 1].inNorm : this.norm;
+        h = hold(ops.linearAddRmsnorm(gpu, g, l.down, x, l.postMlpNorm, next));
+        drop(g);
+      });
+      held.delete(h);
+      return h;
+    } finally {
+      for (const t of held) t.release();
+    }
   }
 
   // One token of every sequence recorded as a HIP graph. Returns { input [batch, 640], output [batch, 640],
@@ -287,7 +299,14 @@ export class Gemma3 {
     const input = gpu.empty([cache.batch, GEMMA.hidden]);
     gpu.write(input.buf, new Float32Array(cache.batch * GEMMA.hidden));
     const pos = gpu.fromArray(new Int32Array(cache.batch).fill(-1), [cache.batch]);
-    const g = gpu.capture(() => this.extendEmbedded(cache, ops.elementwise(gpu, "copy", input), pos, 1));
+    let g;
+    try {
+      g = gpu.capture(() => this.extendEmbedded(cache, ops.elementwise(gpu, "copy", input), pos, 1));
+    } catch (e) {
+      input.release();
+      pos.release();
+      throw e;
+    }
     return {
       input,
       output: g.result,

@@ -8,6 +8,7 @@ const here = path.dirname(fileURLToPath(import.meta.url));
 const js = path.resolve(here, "..", "..", "nanosaur2-web_amd", "js");
 let Gemma3, GEMMA;
 
+// A source of embedding rows that answers when it is told to, and an encoder whose layer stack records its calls.
 function setup(batch, capacity) {
   const live = new Set();
   const tensor = (arr, shape) => {
@@ -35,7 +36,6 @@ function setup(batch, capacity) {
   te.extendEmbedded = (cache, x, pos, L) => {
     ran.push({ pos: Array.from(pos.arr), L, rows: x.shape[0] });
     x.release();
-    if (te.broken) throw new Error("a launch failed");
     return tensor(new Float32Array(1), [1]);
   };
   const cache = { batch, capacity, bits: 16, sinks: 0, layers: [], lengths: new Array(batch).fill(0), cs: [] };
@@ -122,6 +122,44 @@ async function main() {
     s.cache.lengths[0] = 1;
     s.asked.forEach((a) => a.answer());
     out.cut = { ends: await doneAgain, ran: s.ran.slice(1), lengths: [...s.cache.lengths] };
+  }
+  {
+    // the whole layer stack on a device that launches nothing, once for every launch that may fail: which tensors it
+    // keeps, but for those of the op that failed
+    const bf16 = (N, K) => ({ kind: "bf16", buf: { ptr: 1n }, N, K, name: "w" });
+    const i4 = (N, K) => ({ ...bf16(N, K), kind: "i4", scale: { ptr: 1n }, group: 32 });
+    out.failures = {};
+    for (const [kind, W] of [["bf16", bf16], ["i4", i4]]) {
+      const kept = [];
+      let launches = Infinity;
+      for (let n = 0; n <= launches && n < 100; n++) {
+        const live = new Map();
+        let made = 0;
+        let runs = 0;
+        let since = 0; // tensors made before the op that fails
+        const empty = (shape, dtype = "f32") => {
+          const t = { shape, dtype, buf: { ptr: 1n }, get size() { return shape.reduce((a, b) => a * b, 1); }, release() { live.delete(t); } };
+          live.set(t, made++);
+          return t;
+        };
+        const gpu = { empty, fromArray: (arr, shape) => empty(shape), run(name) {
+          if (runs++ === n) throw new Error("a launch failed");
+          if (name !== "te.proj" && name !== "te.mlp") since = made; // (these are the first of an op's two launches)
+        } };
+        const te = new Gemma3(gpu, { rows: async (name, ids) => new Float32Array(ids.length * GEMMA.hidden) });
+        const norms = { inNorm: bf16(1, 1), postAttnNorm: bf16(1, 1), preMlpNorm: bf16(1, 1), postMlpNorm: bf16(1, 1), qn: bf16(1, 1), kn: bf16(1, 1) };
+        const layer = (i) => ({ ...norms, global: i === 1, qkv: W(1536, 640), o: W(640, 1024), gateUp: W(4096, 640), down: W(640, 2048) });
+        te.layers = [layer(0), layer(1)];
+        te.norm = bf16(1, 1);
+        const kv = { batch: 1, KH: 1, D: 256, capacity: 8, ldkv: 256, kvBatch: 2048 };
+        const cache = { batch: 1, capacity: 8, sinks: 0, layers: [kv, kv], lengths: [0], cs: [null, null] };
+        const end = (await ends([te.extend(cache, [1, 2])]))[0];
+        if (end === "ok") launches = n; // every launch has failed once
+        const stay = [...live.values()].filter((at) => end === "ok" || at < since).length;
+        kept.push([end, stay, cache.lengths[0]]);
+      }
+      out.failures[kind] = kept;
+    }
   }
   process.stdout.write(JSON.stringify(out) + "\n");
 }

@@ -45,3 +45,12 @@ def test_a_recorded_step_meets_a_call_in_flight(checks):
     assert c["ends"] == ["ok"] and c["steps"] == [[2]] and [r["pos"] for r in c["ran"]] == [[3, 4]] and c["lengths"] == [5]
     c = checks["cut"]
     assert c["ends"] == ["ok"] and [r["pos"] for r in c["ran"]] == [[1]] and c["lengths"] == [2]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "i4"])
+def test_a_failing_launch_leaves_nothing_behind(checks, kind):
+    """Whichever launch of the layer stack fails: the positions, the activations and the results of the ops before it go
+    back to the pool, and no token counts. The call without a failure keeps its result alone."""
+    runs = checks["failures"][kind]
+    assert len(runs) > 10 and runs[-1] == ["ok", 1, 2], runs
+    assert all(r == ["a launch failed", 0, 0] for r in runs[:-1]), runs
