@@ -218,7 +218,7 @@ export class Gemma3 {
   // order in which they were made, also where none waits for the one before; one that fails adds no token.
   extend(cache, ids) {
     const run = async (before) => {
-      const lists = cache.batch === 1 && !Array.isArray(ids[0]) ? [ids] : ids;
+      const lists = cache.batch === 1 && typeof ids[0] !== "object" ? [ids] : ids;
       const counts = lists.map((t) => t.length);
       const L = Math.max(0, ...counts);
       const padded = [];

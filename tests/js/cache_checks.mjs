@@ -124,6 +124,13 @@ async function main() {
     out.cut = { ends: await doneAgain, ran: s.ran.slice(1), lengths: [...s.cache.lengths] };
   }
   {
+    // token ids as typed arrays, in a list or by themselves
+    const s = setup(1, 16);
+    const done = ends([s.te.extend(s.cache, [Int32Array.of(5, 6, 7)]), s.te.extend(s.cache, Uint16Array.of(8, 9)), s.te.extend(s.cache, [[1]])]);
+    s.asked.forEach((a) => a.answer());
+    out.typed = { ends: await done, ran: s.ran.map((r) => r.pos), asked: s.asked.map((a) => a.ids) };
+  }
+  {
     // the whole layer stack on a device that launches nothing, once for every launch that may fail: which tensors it
     // keeps, but for those of the op that failed
     const bf16 = (N, K) => ({ kind: "bf16", buf: { ptr: 1n }, N, K, name: "w" });

@@ -54,3 +54,7 @@ def test_a_failing_launch_leaves_nothing_behind(checks, kind):
     runs = checks["failures"][kind]
     assert len(runs) > 10 and runs[-1] == ["ok", 1, 2], runs
     assert all(r == ["a launch failed", 0, 0] for r in runs[:-1]), runs
+
+
+def test_ids_in_typed_arrays(checks):
+    assert checks["typed"] == {"ends": ["ok"] * 3, "ran": [[0, 1, 2], [3, 4], [5]], "asked": [[5, 6, 7], [8, 9], [1]]}
