@@ -311,19 +311,15 @@ def _plain_attention(s):
 
 # ---- the framework's calls ------------------------------------------------------------------------
 
-_LIB = None
-
-
 def _lib():
-    """The library on torch's stream: loaded by the first pass, as a program does once."""
-    global _LIB
-    if _LIB is None:
-        sys.path.insert(0, os.path.join(os.getcwd(), "nanosaur2-web_amd"))
-        import ns2
+    pkg = os.path.join(os.getcwd(), "nanosaur2-web_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import ns2
 
-        _LIB = ns2.load(0)
-        _LIB.set_stream(torch.cuda.current_stream().cuda_stream)
-    return _LIB
+    lib = ns2.load(0)
+    lib.set_stream(torch.cuda.current_stream().cuda_stream)
+    return lib
 
 
 def _own_linear(s):
