@@ -260,7 +260,7 @@ export class Gemma3 {
   // The layer stack on new tokens x [batch * L, 640] (released here) at positions pos (int32 on the device).
   // On 4-bit weights the queries, and with them the attention's outputs, are fp16 (each rounded once, as the operands of
   // the whole-prompt encoder's linears are): the linear behind it takes them in one product instead of two, a step of
-  // one token 627 us instead of 703, 200 tokens 1344 instead of 1447. That is 2^-12 of a value, where a weight's code is
+  // one token 627 us instead of 703, 200 tokens 1344 instead of 1447. That is up to 2^-11 of a value, where a weight's code is
   // off by up to a fourteenth of its group's largest.
   extendEmbedded(cache, x, pos, L) {
     const gpu = this.gpu;
