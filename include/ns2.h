@@ -295,8 +295,9 @@ int ns2_attention_rows_f16kv_oproj(const float* q, const uint16_t* k, const uint
  *   j < sinks or j > p - window (window = 0: all j <= p).
  * What the cache holds at other positions, infinities and NaN too, does not matter. kvBatch = 0 lets
  * all sequences read one cache. The softmax weights, and fp32 queries, take part as sums of fp16
- * parts that keep 22 of their bits (of a query value below 2^-16 of its head's largest, fewer).
- * o must not overlap q.
+ * parts that keep 21 of their bits (of a query value below 2^-16 of its head's largest, fewer).
+ * Infinities and NaN in visible keys and values act as the formula says (an infinite value whose
+ * weight is below 2^-29 of the row's largest may give NaN). o must not overlap q.
  * Sums and softmax statistics are fp32; the same call gives the same bits again. work:
  * ns2_attention_cache_bytes bytes of device memory that the call may write (NULL where that is 0);
  * calls that may overlap take one each. */

@@ -18,6 +18,7 @@ namespace ns2cache {
 using namespace ns2dev;
 
 typedef float float2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kGroup = 32;  // values per step and offset of a 4-bit cache
@@ -177,7 +178,7 @@ __device__ __forceinline__ int qdim(int t, int grp) {
 }
 
 // Column m's query (zeros for padding), negated for a negative scale. fp32 queries are scaled by a power of two to
-// below 2^14 and taken as two halves that keep 22 bits.
+// below 2^14 and taken as two halves that keep 21 bits.
 template <int D, bool I4, bool F32>
 struct Query {
   static constexpr int QT = D / 32;
@@ -226,9 +227,13 @@ struct Query {
       const float y[8] = {x[t][0].x, x[t][0].y, x[t][0].z, x[t][0].w, x[t][1].x, x[t][1].y, x[t][1].z, x[t][1].w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float z = ldexpf(sign * y[order[e]], up);
-        hi[e] = (half_t)z;
-        lo[e] = (half_t)(z - (float)hi[e]);
+        // both of z's sign unless it is 0 (they are fp16's smallest at least, 2^-38 of the largest), so that two products
+        // with an infinity agree
+        const float z = ldexpf(sign * y[order[e]], up), least = z == 0.f ? 0.f : copysignf(0x1p-24f, z);
+        const half_t h = (half_t)__builtin_amdgcn_cvt_pkrtz(z, z)[0];
+        const half_t l = (half_t)(z - (float)h);
+        hi[e] = h == (half_t)0.f ? (half_t)least : h;
+        lo[e] = h == (half_t)0.f || l == (half_t)0.f ? (half_t)least : l;
       }
     }
   }
@@ -271,18 +276,20 @@ __device__ __forceinline__ float4_t mfma(half4_t a, half4_t b, float4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
 }
 
-// The B operand of the second product: the weights as two halves that keep 22 bits, the second what the first's
-// rounding left (one mixed-precision multiply-add; the factor hides from the compiler, which would make a conversion
-// and a subtraction of it). For fp16 queries too: with one half per weight, the sum of weights that divides the
-// output would have to be one of rounded weights, and the output's error is half as large again as that of its own
-// rounding (2.9e-4 against 2.1e-4).
+// The B operand of the second product: the weights as two halves that keep 21 bits, the first one step below the weight
+// cut off, the second what that left (one mixed-precision multiply-add; the factor hides from the compiler, which would
+// make a conversion and a subtraction of it). For fp16 queries too: with one half per weight, the sum of weights that
+// divides the output would have to be one of rounded weights, and the output's error is half as large again as that of
+// its own rounding (2.9e-4 against 2.1e-4). Both halves are positive where the weight is (from 2^-23 on, 2^-29 of the
+// weight of the reference), so that two products with an infinity agree.
 template <int N, class H>
 __device__ __forceinline__ void weights(const float (&p)[N], H& hi, H& lo) {
   float one = 1.f;
   asm("" : "+s"(one));
 #pragma unroll
   for (int e = 0; e < N; e += 2) {
-    const half2_t h = __builtin_convertvector(float2_t{p[e], p[e + 1]}, half2_t);
+    const ushort2_t u = __builtin_bit_cast(ushort2_t, __builtin_amdgcn_cvt_pkrtz(p[e], p[e + 1]));
+    const half2_t h = __builtin_bit_cast(half2_t, __builtin_elementwise_sub_sat(u, ushort2_t{1, 1}));
     const half2_t l = __builtin_convertvector(
         float2_t{__builtin_fmaf(-(float)h[0], one, p[e]), __builtin_fmaf(-(float)h[1], one, p[e + 1])}, half2_t);
     hi[e] = h[0];

@@ -11,7 +11,7 @@
 // 16-byte slots inside one are exchanged (xor) by a pattern of the fragment so that the threads of a row write to
 // different banks.
 //
-// Measured: 2 x 3001 fp32 queries of 16 heads of 128 on 1003 to 4003 4-bit keys of 4 heads 248 us (382 TFLOP/s, and
+// Measured: 2 x 3001 fp32 queries of 16 heads of 128 on 1003 to 4003 4-bit keys of 4 heads 254 us (373 TFLOP/s, and
 // twice that in products, since fp32 takes two), 4096 fp16 queries of 4 heads of 256 in a window of 512 28 us (290
 // TFLOP/s, and half as much again in products: the weights take two). A tile of the first takes a wave about 5100 cycles, of which 2048 keep the matrix cores busy; the rest is
 // mostly VALU work of the two waves of a SIMD (300 instructions each: 4-bit values 115, softmax and weights 130).

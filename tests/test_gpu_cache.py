@@ -869,3 +869,47 @@ def test_queries_beside_the_rows(ns2lib, fp16):
         torch.cuda.synchronize()
         q = torch.as_strided(buf, (L, per), (ldq, 1), q0).contiguous().view(dt)
         assert torch.equal(q, own) and torch.equal(x, data) and all(torch.equal(m, n) for m, n in zip(got, want))
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("L", [1, 5, 70, 300])
+def test_visible_infinities(ns2lib, L, D, i4, fp16):
+    """What is not finite in keys and values that are visible does what it does in 64 bits: a value of +-inf makes that
+    dimension +-inf, both of them or a NaN make it NaN, a key whose score is -inf weighs nothing, and the dimensions and
+    rows that meet none of it stay within the usual bound."""
+    cap, H, KH = 700, 4, 2
+    rnd = gen(63 + D)
+    cache = Cache(rnd, 1, cap, KH, D, i4)
+    pos = positions([(cap - L - 20, L)], L)
+    q = rnd(1, L, H, D)
+    q[..., 7] = q[..., 7].abs() + 0.5
+
+    def put(name, key, head, dim, x):
+        if i4:  # the offset of the dimension's group
+            cache.group_view(name)[0, key, head, dim // 32, 1] = x
+            cache.value[name][0, key, head, dim // 32 * 32: dim // 32 * 32 + 32] = x
+        else:
+            cache.view(cache.raw[name], 1)[0, key, head, dim] = x
+            cache.value[name][0, key, head, dim] = x
+
+    late = cap - 20 - L // 2 - 1  # (seen by the later rows only)
+    for key, head, dim, x in ((40, 0, 3, math.inf), (333, 1, 5, -math.inf), (100, 1, D - 1, math.inf), (200, 1, D - 2, -math.inf),
+                              (late, 0, D - 3, math.nan), (late, 1, 5, -math.inf)):
+        put("v", key, head, dim, x)
+    if not i4:  # scores of -inf: one key far from the others, and eight in a row
+        for key in (77, *range(160, 168)):
+            put("k", key, 0, 7, -math.inf)
+            put("k", key, 1, 7, -math.inf)
+    for window, sinks in ((0, 0), (400, 90)):
+        got = attend(ns2lib, cache, q, pos, window, sinks, fp16)[0].double()
+        qd = (q.half() if fp16 else q).double()
+        ref = R.attention(qd, pos, cache.value["k"], cache.value["v"], window, sinks, 1 / math.sqrt(D))[0][0]
+        kinds = [torch.where(torch.isnan(t), 2.0, torch.where(torch.isinf(t), t.sign(), 0.0)) for t in (got, ref)]
+        assert torch.equal(*kinds), f"window {window}: {(kinds[0] != kinds[1]).sum().item()} of {got.numel()} outputs of another kind"
+        k, v = (torch.where(torch.isfinite(cache.value[n]), cache.value[n], 0.0) for n in "kv")
+        _, vmax, smax, n = R.attention(qd, pos, k, v, window, sinks, 1 / math.sqrt(D))
+        bound = R.attention_bound(torch.where(torch.isfinite(ref), ref, 0.0), vmax, smax, n, D, fp16)[0]
+        fine = torch.isfinite(ref)
+        assert ((got - ref).abs() <= bound)[fine].all()
