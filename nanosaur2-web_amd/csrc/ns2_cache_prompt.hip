@@ -13,8 +13,9 @@
 //
 // Measured: 2 x 3001 fp32 queries of 16 heads of 128 on 1003 to 4003 4-bit keys of 4 heads 254 us (373 TFLOP/s, and
 // twice that in products, since fp32 takes two), 4096 fp16 queries of 4 heads of 256 in a window of 512 28 us (290
-// TFLOP/s, and half as much again in products: the weights take two). A tile of the first takes a wave about 5100 cycles, of which 2048 keep the matrix cores busy; the rest is
-// mostly VALU work of the two waves of a SIMD (300 instructions each: 4-bit values 115, softmax and weights 130).
+// TFLOP/s, and half as much again in products: the weights take two). A tile of the first takes a wave about 5200
+// cycles, of which 2048 keep the matrix cores busy; the rest is mostly VALU work of the two waves of a SIMD (300
+// instructions each: 4-bit values 115, softmax and weights 134).
 // Heads of 256 are bound by LDS: their 64 columns read each fragment four times (2048 of 4000 cycles). Four waves of
 // 32 columns, which read it twice, leave a SIMD one wave and took 39 us.
 #include "ns2_cache.h"

@@ -913,3 +913,48 @@ def test_visible_infinities(ns2lib, L, D, i4, fp16):
         bound = R.attention_bound(torch.where(torch.isfinite(ref), ref, 0.0), vmax, smax, n, D, fp16)[0]
         fine = torch.isfinite(ref)
         assert ((got - ref).abs() <= bound)[fine].all()
+
+
+@pytest.mark.parametrize("i4", [False, True])
+@pytest.mark.parametrize("L", [3, 80])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+def test_queries_of_each_magnitude(ns2lib, D, L, i4):
+    """fp32 queries of one magnitude per call, far below and beyond fp16's range, with a scale that makes their scores
+    those of ordinary queries: the bound is small beside the values (asserted), so that a wrong query shows."""
+    rnd = gen(64 + D + L)
+    pos = positions([(60, L), (0, L)], L)
+    cache = Cache(rnd, 2, 160, 2, D, i4)
+    base = rnd(2, L, 4, D)
+    for f in (1e-30, 1e-20, 1e-7, 1e-3, 1.0, 3e2, 1e4, 1e12, 1e30):
+        q, scale = base * f, 1 / (f * math.sqrt(D))
+        got = attend(ns2lib, cache, q, pos, 0, 0, False, scale=scale)
+        # (the scale as the call takes it, in 32 bits)
+        ref, vmax, smax, n = R.attention(q.double(), pos, cache.value["k"], cache.value["v"], 0, 0, float(torch.tensor(scale, dtype=torch.float32)))
+        bound = R.attention_bound(ref, vmax, smax, n, D, False)
+        live = (pos >= 0)
+        assert (bound[live] < 1e-2 * vmax[live]).all()
+        err = (got[live].double() - ref[live]).abs()
+        print(f"[parity] D={D} L={L} i4={i4} x {f}: largest error / bound {(err / bound[live]).max().item():.3f}", flush=True)
+        assert (err <= bound[live]).all(), f
+
+
+@pytest.mark.parametrize("fp16", [False, True])
+@pytest.mark.parametrize("L", [1, 90])
+def test_scores_that_are_all_minus_infinity(ns2lib, L, fp16):
+    """A row all of whose scores are -inf has no softmax: NaN, in its own heads; where one key is left, the row is that
+    key's value."""
+    rnd = gen(65)
+    D, cap = 128, 400
+    cache = Cache(rnd, 2, cap, 2, D, False)
+    k = cache.view(cache.raw["k"], 1)
+    k[:, :, :, 0] = -math.inf
+    k[1, 17, 0, 0] = 1.0  # (sequence 1, head 0: one key is left)
+    q = rnd(2, L, 4, D)
+    q[..., 0] = 1.0
+    pos = positions([(cap - L, L)] * 2, L)
+    got = attend(ns2lib, cache, q, pos, 0, 0, fp16)
+    assert torch.isnan(got[0]).all() and torch.isnan(got[1, :, 2:]).all()
+    want = cache.value["v"][1, 17, 0]
+    err = (got[1, :, :2].double() - want).abs()
+    # one weight in 21 bits over itself, two sums, the output's rounding
+    assert (err <= want.abs() * (2.0**-21 + 2.0**-22 + (2.0**-11 if fp16 else 2.0**-23)) + 2.0**-24).all()

@@ -173,3 +173,18 @@ def test_calls_in_flight_and_steps_of_one_sequence(model, bits):
     assert p.returncode == 0, p.stderr[-2000:]
     got = json.loads(p.stdout.strip().splitlines()[-1])
     assert got == {"overlap": 0, "recorded": 0, "lengths": [[6, 6], [6, 6], [9, 9], [9, 9]]}
+
+
+@pytest.mark.parametrize("chunk", [1, 9])
+def test_loras_over_a_cache(model, chunk):
+    """LoRAs on the encoder's linears act on tokens in pieces as on the whole prompt (which is held to the goldens)."""
+    from safetensors.torch import save_file
+
+    lora = str(model[2] / "te_lora.safetensors")
+    save_file(G.make_te_lora(), lora)
+    ids = G.make_ids(21, seed=51)
+    whole = hidden(model, ids, "--lora", lora + ":0.8")
+    got = hidden(model, ids, "--cache", 32, "--chunk", chunk, "--lora", lora + ":0.8")
+    assert_close(got, whole, 1e-2, f"LoRA in pieces of {chunk}")
+    plain = hidden(model, ids, "--cache", 32, "--chunk", chunk)
+    assert (got - plain).norm() > 1e-2 * plain.norm(), "the LoRA changes less than the tolerance"
