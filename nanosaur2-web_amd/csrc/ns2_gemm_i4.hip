@@ -87,7 +87,7 @@ constexpr int pieces() {
   return WK == 16 ? 2 : 6;
 }
 // Places of a piece of 8 columns in LDS: an odd number, since threads that write pieces of one row would meet in the
-// same banks otherwise (16 x 4096 x 1536 fp32 8.7 us, so 7.2).
+// same banks otherwise (16 x 4096 x 1536 fp32 8.7 us, so 7.3).
 __host__ __device__ constexpr int places(int rows) { return rows | 1; }
 
 // A block takes 16 RT rows and, with WK = 1, 64 CT columns (16 CT per wave) over all of K; with WK = 4 or 16, 16 CT
@@ -101,6 +101,7 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
   extern __shared__ __attribute__((aligned(16))) char smem[];
   half8_t* x_s = reinterpret_cast<half8_t*>(smem);
   __shared__ uint32_t top_s[16 * RT];
+  __shared__ int infinite_s;  // a row of the slab holds an infinity
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c16 = lane & 15, g = lane >> 4;
   const int m0 = blockIdx.y * (16 * RT);
@@ -155,6 +156,7 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
       constexpr int NI = pieces<WK>();
       float4 x[NI][2];
       for (int u = threadIdx.x; u < rows; u += 64 * kWaves) top_s[u] = 0u;
+      if (threadIdx.x == 0) infinite_s = 0;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int u = threadIdx.x + 64 * kWaves * i, r = u / n8, k8 = u - r * n8;
@@ -166,27 +168,37 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
         }
       }
       __syncthreads();
-      // magnitudes order as their bits do; four neighbours share a row (n8 is a multiple of 4). What is finite decides
-      // the scaling.
-      uint32_t infinite = 0;  // pieces that hold an infinity
+      // magnitudes order as their bits do; four neighbours share a row (n8 is a multiple of 4)
+      bool infinite = false;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int u = threadIdx.x + 64 * kWaves * i;
         const float4 a = x[i][0], b = x[i][1];
         float top = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
                           fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
-        if (top == INFINITY) {
-          infinite |= 1u << i;
-          const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-          top = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
-        }
+        infinite |= top == INFINITY;
         top = fmaxf(top, dpp<kDppXor1>(top));
         top = fmaxf(top, dpp<kDppXor2>(top));
         if (u < items && (threadIdx.x & 3) == 0) atomicMax(&top_s[u / n8], __builtin_bit_cast(uint32_t, top));
       }
+      if (infinite) infinite_s = 1;
       __syncthreads();
+      infinite = __builtin_amdgcn_readfirstlane(infinite_s) != 0;
+      if (infinite) {  // what is finite decides the scaling
+        for (int u = threadIdx.x; u < rows; u += 64 * kWaves) top_s[u] = 0u;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int u = threadIdx.x + 64 * kWaves * i;
+          const float4 a = x[i][0], b = x[i][1];
+          const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+          float top = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
+          if (u < items) atomicMax(&top_s[u / n8], __builtin_bit_cast(uint32_t, top));
+        }
+        __syncthreads();
+      }
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int u = threadIdx.x + 64 * kWaves * i, r = u / n8, k8 = u - r * n8;
@@ -201,7 +213,7 @@ __global__ __launch_bounds__((64 * waves<WK>())) void linear_i4_kernel(I4Args p)
             hi[e] = (half_t)t;
             lo[e] = (half_t)(t - (float)hi[e]);
           }
-          if (infinite >> i & 1) {  // an infinity is all in hi
+          if (infinite) {  // an infinity is all in hi
 #pragma unroll
             for (int e = 0; e < 8; ++e) lo[e] = fabsf(v[e]) == INFINITY ? (half_t)0.f : lo[e];
           }
@@ -337,15 +349,15 @@ void launch_i4(const I4Args& p, hipStream_t s) {
 }
 
 // By the number of 16 x 16 tiles of the output (us, "a | b": fp16 | fp32 x):
-//  - many tiles: all of K in a wave of 32 columns, loads two chunks ahead (256 x 4096 x 640 9.9 | 11.2, over four
-//    waves 10.9 | 18.3; 12 x 32768 x 2048 16.7 | 18.7, 18.4 | 24.5); with up to four fp16 rows, whose products cost
+//  - many tiles: all of K in a wave of 32 columns, loads two chunks ahead (256 x 4096 x 640 9.9 | 11.3, over four
+//    waves 10.9 | 18.3; 12 x 32768 x 2048 16.7 | 18.9, 18.4 | 24.5); with up to four fp16 rows, whose products cost
 //    least, 16 columns and loads four chunks ahead (1 x 262144 x 640 18.2, with 32 columns 19.9); with many fp16 rows
 //    32 of them per block, unless that leaves an eighth of the blocks' rows empty (32 x 65536 x 2048 34.5, with 16
 //    50; 300 x 27000 x 1536 82, 102; 48 x 65600 x 640 26.9, 24.4. fp32 rows take the same either way, 128 and 131);
 //  - few tiles and a K that gives sixteen waves work: over sixteen waves (1 x 8192 x 1536 4.1 | 4.8, over four 4.6 |
 //    4.9; 16 x 8192 x 1536 5.3 | 8.2, 7.3 | 10.0), of 16 columns up to one block per CU or where rows cost least
-//    (16 x 4096 x 1536 fp32 7.3, with 32 columns 7.9), else of 32 (16 x 8192 x 1536 fp32 8.2, with 16 12.6);
-//  - between: over four waves of 32 columns (8 x 16384 x 4096 fp32 21, with 16 columns 28.6; in one wave 27.8).
+//    (16 x 4096 x 1536 fp32 7.4, with 32 columns 7.9), else of 32 (16 x 8192 x 1536 fp32 8.2, with 16 12.6);
+//  - between: over four waves of 32 columns (8 x 16384 x 4096 fp32 21.4, with 16 columns 28.6; in one wave 27.8).
 // The bytes bound a table (1 x 262144 x 640: 90 MB at 5.0 TB/s); the smallest calls are a launch and two round trips
 // to memory; many rows are bound by the VALU, which decodes the weights again for every block of rows (300 x 27000 x
 // 1536: 300 TFLOP/s, fp32 190).
