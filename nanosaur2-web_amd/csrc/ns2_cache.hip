@@ -283,7 +283,11 @@ __global__ __launch_bounds__(256) void cache_join_kernel(AttnArgs a) {
     *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = make_float4(q.x * inv, q.y * inv, q.z * inv, q.w * inv);
 }
 
-constexpr int kRowsColumns = 64;  // columns of a K/V head up to which its keys are streamed past 16 at a time
+// Columns of a K/V head up to which its keys are streamed past 16 at a time, though they are read again for every 16.
+// us, streamed | tiles in LDS: 8 sequences of 4 fp16 heads of 256 on 4096 fp16 keys, 32 columns 18.5 | 18.8, 64 21.9 |
+// 22.6, 80 25.1 | 22.7, 128 30.9 | 25.2; 16 heads of 128 over 4 4-bit ones, 32 20.2 | 27.6, 64 28.1 | 29.7, 80 34.6 |
+// 35.3, 96 45.9 | 36.2; fp32 queries and long caches of few sequences gain a little more by streaming.
+constexpr int kRowsColumns = 64;
 constexpr long long kCUs = 256;
 
 Plan plan_of(int batch, int L, int H, int KH, int cap, int window, int sinks) {
