@@ -86,12 +86,12 @@ __device__ __forceinline__ uint32_t codes_of(const double (&y)[4], half_t& step,
 // time: the sum of squares runs over units of 8 lanes (DPP) and then over the head's D / 32 units, the rotation's
 // partner i +- D/2 is D / 8 lanes away, and a 4-bit group is one unit of 8 lanes. Every value is read once and
 // written once, which bounds it; U times as many heads per wave, all asked for at once, keep the memory busy
-// where there are enough of them (8191 tokens x 24 heads of 128 to fp16: 30.6 us with one, 29.7, 5.2 TB/s, with
-// four; 2048 tokens 9.0, 9.8).
+// where there are enough of them (8191 tokens x 24 heads of 128 to fp16, the same rows again: 30.6 us with one, 29.7
+// with four; rows that come from memory 35.6, 4.3 TB/s; 2048 tokens 9.0, 9.8).
 //
 // What becomes 4-bit codes is computed in 64 bits, keys from the norm on: a value's last bits in fp32 would decide
-// between two codes, a step of the whole value apart, wherever it lies near their border. 2400 tokens x 6 heads of 256
-// 8.8 us, in fp32 7.4.
+// between two codes, a step of the whole value apart, wherever it lies near their border. (Value heads go through the
+// norm's sums with the keys and leave the result.) 2400 tokens x 6 heads of 256 8.4 us, in fp32 7.4.
 template <int D, bool I4, int U>
 __global__ __launch_bounds__(256) void cache_write_kernel(WriteArgs a) {
   constexpr int T = D / 4, HPW = 256 / D;

@@ -16,8 +16,9 @@
 // TFLOP/s, and half as much again in products: the weights take two). A tile of the first takes a wave about 5200
 // cycles, of which 2048 keep the matrix cores busy; the rest is mostly VALU work of the two waves of a SIMD (300
 // instructions each: 4-bit values 115, softmax and weights 134).
-// Heads of 256 are bound by LDS: their 64 columns read each fragment four times (2048 of 4000 cycles). Four waves of
-// 32 columns, which read it twice, leave a SIMD one wave and took 39 us.
+// Heads of 256 wait for LDS most: their 64 columns read each fragment four times (2048 of about 4400 cycles a tile,
+// products 1536). Four waves of 32 columns, which read it twice, leave a SIMD one wave and took 39 us (with weights
+// of one half, where the kernel took 26).
 #include "ns2_cache.h"
 
 using namespace ns2cache;

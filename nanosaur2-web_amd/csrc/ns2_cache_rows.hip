@@ -10,7 +10,7 @@
 // Measured, with the join of the splits: 16 fp16 tokens of 16 heads on 16384 fp16 keys of 4 heads of 128 98 us (the
 // cache at 5.5 TB/s, a copy reads and writes 5.2); 32 tokens of 4 heads on up to 16000 4-bit keys of one head of 256
 // 38 us (2.9 TB/s: eight 4-bit values of a lane take 13 instructions, the VALU is busy 60 % of the time); one fp32
-// token on a window of 516 fp16 keys of 256 10.4 us, the chain of two launches (position, keys, merge; sums, output).
+// token on a window of 516 fp16 keys of 256 10.6 us, the chain of two launches (position, keys, merge; sums, output).
 #include "ns2_cache.h"
 
 using namespace ns2cache;
