@@ -284,11 +284,11 @@ int ns2_attention_rows_f16kv_oproj(const float* q, const uint16_t* k, const uint
  * (a q|k|v product). Query and key heads are RMS-normed with w_q / w_k [D] (NULL: not normed) and,
  * for positions below rope_rows, rotated by the table cs at their position (ns2_head_norm's
  * layout; NULL: not rotated). Queries go to q [batch*L, ldq]: X itself (fp32 with ldq == ldx), rows
- * beside X's in one buffer, or memory of their own; any other overlap with X is refused. Keys and
- * values go into the cache at their rows' positions, which have to differ within a sequence. A
- * 4-bit group takes o = half(least value), s = half(range / 15), code = clamp(rint((x - o) / s), 0,
- * 15), with norm, rotation and codes in 64 bits; a group that holds a NaN or an infinity reads as
- * NaN. The sequences' caches must not overlap, nor any of them X or q.
+ * beside X's in one buffer, as many bytes apart as X's, or memory of their own; any other overlap
+ * with X is refused. Keys and values go into the cache at their rows' positions, which have to
+ * differ within a sequence. A 4-bit group takes o = half(least value), s = half(range / 15), code =
+ * clamp(rint((x - o) / s), 0, 15), with norm, rotation and codes in 64 bits; a group that holds a
+ * NaN or an infinity reads as NaN. The sequences' caches must not overlap, nor any of them X or q.
  *
  * ns2_attention_cache: for each row at position p, head h and g = h / (H / KH),
  *   o[row*ldo + h*D ..] = sum_j softmax_j(scale * <q_row,h, k_j,g>) v_j,g over the keys j <= p with
